@@ -31,6 +31,7 @@ OPS = {
 _lib = None
 _dev = None
 _V, _I64, _I, _F, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_D = ctypes.c_double
 
 _SIGS = {
     "euc_version": ([], ctypes.c_char_p),
@@ -64,6 +65,16 @@ _SIGS = {
     "euc_center_stats_workspace_bytes": ([_I64, _I64, _I64], _SZ),
     "euc_center_stats": ([_V, _I, _V, _I, _I64, _I64, _I64, _V, _V, _SZ, _V], _I),
     "euc_center_finalize": ([_V, _I64, _I64, _V, _I, _V, _I, _V], _I),
+    "euc_label_log_probs": ([_I, _V, _I64, _I64, _I64, _V, _I, _D, _I, _V, _V, _V, _V, _V, _V], _I),
+    "euc_label_log_probs_grad": ([_I, _V, _I64, _I64, _I64, _V, _I, _D, _V, _V, _V, _V, _V], _I),
+    "euc_group_rows_workspace_bytes": ([_I64, _I64], _SZ),
+    "euc_group_rows": ([_V, _I, _I64, _I64, _V, _V, _V, _V, _V, _SZ, _V], _I),
+    "euc_rows_to_groups": ([_I, _V, _V, _V, _I64, _I64, _I64, _V, _V], _I),
+    "euc_rows_from_groups": ([_I, _V, _V, _V, _I64, _I64, _I64, _V, _V], _I),
+    "euc_rows_from_groups_grad": ([_I, _V, _V, _V, _V, _V, _I64, _I64, _I64, _V, _V, _V], _I),
+    "euc_codebook_lookup": ([_I, _V, _I64, _V, _I, _I64, _I64, _D, _V, _V], _I),
+    "euc_codebook_grad_workspace_bytes": ([_I, _I64, _I64], _SZ),
+    "euc_codebook_grad": ([_I, _V, _V, _V, _V, _I64, _I64, _I64, _D, _V, _V, _SZ, _V], _I),
     "euc_kmeanspp_workspace_bytes": ([_I64, _I64, _I64], _SZ),
     "euc_kmeanspp": ([_V, _I, _I64, _I64, _I64, ctypes.c_uint64, _V, _V, _V, _SZ, _V], _I),
 }
@@ -123,6 +134,13 @@ def stream_of(t):
 
 def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+def call_on(t, fn, *args):
+    """fn(*args, stream) on t's device and its current stream, the caller's current device
+    left as it was; tensors are passed as addresses (data_ptr(), None for absent ones)."""
+    with torch.cuda.device(t.device):
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
 
 
 def workspace(nbytes, device):

@@ -13,7 +13,7 @@ import ctypes
 
 import torch
 
-from _lib import OPS, check, lib, ptr, stream_of, workspace
+from _lib import OPS, check, exported_symbols, lib, ptr, stream_of, workspace
 
 _TORCH_DT = {"fp32": torch.float32, "fp64": torch.float64, "fp16": torch.float16, "bf16": torch.bfloat16}
 _DT_NAME = {torch.float32: "float32", torch.float64: "float64", torch.float16: "float16",
@@ -187,6 +187,58 @@ def run_argmin(op_name, P, C, kappa=5.0, exact=False, labels_dtype=torch.int64, 
                            ptr(l64), ptr(l32),
                            ptr(md), ptr(cnt), ptr(ws), ws.numel(), st))
     return labels, md, cnt[0]
+
+
+def run_distance(op_name, P, C, kappa=5.0):
+    """D of any distance operator by its key in _lib.OPS (the default tile size)."""
+    if op_name in ("single", "double"):
+        return run_plain("euc_pairwise_" + op_name, op_name, P, C, _TORCH_DT["fp32" if op_name == "single" else "fp64"])
+    if op_name.startswith("tiled_"):
+        return run_tiled(op_name[len("tiled_"):], P, C, kappa, 0, False)
+    if op_name.startswith("tensorcore_"):
+        return run_tensorcore(op_name[len("tensorcore_"):], P, C, kappa, 0)
+    if "euc_mix_" + op_name not in exported_symbols():
+        raise RuntimeError(f"{op_name}: not a distance operator of the Lloyd loop")
+    return run_mix(op_name, P, C, kappa, False)
+
+
+# euc_row_type of the label operators
+ROW_TYPES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
+
+
+def row_type(t, name):
+    if t.dtype not in ROW_TYPES:
+        raise RuntimeError(f"{name} must be float32, float64, float16 or bfloat16")
+    return ROW_TYPES[t.dtype]
+
+
+def acc_dtype(t):
+    """The type of sums, weights and statistics of rows of t's type."""
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def check_same_device(t, name, other, other_name):
+    if t.device != other.device:
+        raise RuntimeError(f"{name} and {other_name} must be on the same device")
+
+
+def check_labels(labels, name="labels"):
+    """Labels of the label operators: a contiguous int64 or int32 CUDA tensor; returns
+    the C ABI's labels_are_i64."""
+    check_input(labels, name)
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"{name} must be int64 or int32")
+    return int(labels.dtype == torch.int64)
+
+
+def check_like(t, name, shape, dtype, device):
+    check_input(t, name)
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {_DT_NAME[dtype]}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must have shape {tuple(shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}")
 
 
 def read_count_i32(t):

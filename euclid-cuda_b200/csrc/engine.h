@@ -222,6 +222,52 @@ size_t seed_ws_bytes(int64_t n);
 cudaError_t launch_kmeanspp(const void* X, bool x_f64, int64_t n, int64_t dim, int64_t k, uint64_t seed,
                             int64_t* idx, void* centers, void* ws, cudaStream_t st);
 
+// Element type of the label operators (euc_row_type in include/euclid_b200.h).
+enum RowType { ROW_F32 = 0, ROW_F64 = 1, ROW_F16 = 2, ROW_BF16 = 3 };
+
+// Rows sorted by label and back (k_groups.cu).
+size_t group_ws_bytes(int64_t slots, int64_t k);
+cudaError_t launch_group_rows(const void* labels, bool labels_i64, int64_t slots, int64_t k, int32_t* offsets,
+                              int32_t* order, int32_t* position, int32_t* sorted, void* ws, cudaStream_t st);
+cudaError_t launch_rows_to_groups(int esize, const void* X, const int32_t* position, const int32_t* kept, int64_t n,
+                                  int p, int64_t dim, void* Y, cudaStream_t st);
+cudaError_t launch_rows_from_groups(RowType t, const void* Z, const int32_t* position, const void* weights, int64_t n,
+                                    int p, int64_t dim, void* out, cudaStream_t st);
+cudaError_t launch_rows_from_groups_grad(RowType t, const void* G, const void* Z, const int32_t* position,
+                                         const void* weights, const int32_t* kept, int64_t n, int p, int64_t dim,
+                                         void* gZ, void* gW, cudaStream_t st);
+
+// Codebook lookup and its gradient by sorted labels (k_codebook.cu).
+cudaError_t launch_codebook_lookup(RowType t, const void* C, int64_t k, const void* labels, bool labels_i64, int64_t n,
+                                   int64_t dim, double scale, void* out, cudaStream_t st);
+size_t codebook_grad_ws_bytes(RowType t, int64_t n, int64_t dim);
+cudaError_t launch_codebook_grad(RowType t, const void* G, const int32_t* offsets, const int32_t* order,
+                                 const int32_t* sorted, int64_t n, int64_t k, int64_t dim, double scale, void* out,
+                                 void* ws, cudaStream_t st);
+
+// Log probabilities of rows of scores (k_scores.cu); n, m >= 1, top <= m.
+struct ScoreJob {
+  const void* x;
+  int64_t ld, n, m;
+  const void* labels;
+  bool labels_i64;
+  double scale;
+  int top;
+  void *log_probs, *entropy, *stats, *top_log_probs;  // nullable but for the alternatives with top > 0
+  int64_t* top_labels;
+};
+struct ScoreGradJob {
+  const void* x;
+  int64_t ld, n, m;
+  const void* labels;
+  bool labels_i64;
+  double scale;
+  const void *stats, *g_log_probs, *g_entropy;
+  void* grad;
+};
+cudaError_t launch_label_log_probs(RowType t, const ScoreJob& j, cudaStream_t st);
+cudaError_t launch_label_log_probs_grad(RowType t, const ScoreGradJob& j, cudaStream_t st);
+
 // Bound of the pipeline waits of the tensor-core kernels (api.cu, euc_set_wait_limit_ns),
 // and the one-shot failure injection of euc_test_withhold_arrival: true once per arming.
 unsigned long long wait_limit_ns();

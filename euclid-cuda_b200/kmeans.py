@@ -20,6 +20,8 @@ import torch
 import torch.distributed as dist
 
 import _ops
+import codebook
+from label_scores import LabelLogProbs, label_log_probs
 from _lib import check, lib, ptr, stream_of, workspace
 
 EMPTY_POLICY = {"zero": 0, "keep": 1}
@@ -94,6 +96,27 @@ class LloydKMeans:
         labels, _, cnt = _ops.run_argmin(self.op, X, C, self.kappa, exact=self.mode, labels_dtype=torch.int32,
                                          min_dist=False, prepared=prepared)
         return labels, cnt
+
+    def posterior(self, X, C, temperature=1.0, labels=None, top=1, block_rows=None):
+        """Soft assignment of the local rows: LabelLogProbs of -D / temperature, D the
+        operator's squared distances, formed in blocks of `block_rows` rows (default:
+        about 1 GiB of D) so that D is never whole.  `labels`: labels whose log
+        probabilities are wanted; `top`: the nearest centers per row, with theirs."""
+        if not temperature > 0:
+            raise RuntimeError("temperature must be positive")
+        n, m = X.size(0), C.size(0)
+        rows = int(block_rows) if block_rows else max(1, (1 << 30) // max(1, m * X.element_size()))
+        parts = []
+        for lo in range(0, n, rows) if n > 0 else (0,):
+            D = _ops.run_distance(self.op, X[lo:lo + rows], C, self.kappa)
+            parts.append(label_log_probs(D, None if labels is None else labels[lo:lo + rows], -1.0 / temperature, top))
+        if len(parts) == 1:
+            return parts[0]
+        return LabelLogProbs(*(None if f[0] is None else torch.cat(f) for f in zip(*parts)))
+
+    def reconstruct(self, C, labels, scale=1.0):
+        """The rows that the labels stand for: scale * C[labels] (codebook.lookup)."""
+        return codebook.lookup(C, labels, scale)
 
     def step(self, X, C, prepared=None):
         """One iteration on the local shard X; returns (new centers, labels int32,

@@ -334,6 +334,72 @@ EUC_API size_t euc_kmeanspp_workspace_bytes(int64_t n, int64_t dim, int64_t k);
 EUC_API int euc_kmeanspp(const void* X, int x_is_f64, int64_t n, int64_t dim, int64_t k, uint64_t seed,
                  int64_t* indices, void* centers, void* ws, size_t ws_bytes, void* stream);
 
+/* ---------------------------------------------------------- label operators
+ * No counterpart in the reference.  What a caller does with labels: how sure a label
+ * is, rows brought together by label and back, and codebook rows from labels; each
+ * with its gradient.  All results are the same on every run (no atomics on values).
+ * Sums, weights and statistics are fp32, and fp64 for fp64 rows. */
+typedef enum { EUC_ROW_F32 = 0, EUC_ROW_F64 = 1, EUC_ROW_F16 = 2, EUC_ROW_BF16 = 3 } euc_row_type;
+
+/* Log probabilities of n rows of m scores (row stride ld >= m elements), z = scale * x:
+ * a row of D of any distance operator takes scale = -1 / temperature.
+ *   log_probs[i]     = z[i, l_i] - log sum_j exp z[i, j]   (0 where l_i is outside [0, m))
+ *   entropy[i]       = - sum_j p_j log p_j
+ *   top_log_probs, top_labels (n x top): the largest of z, equal ones by the lower
+ *                      index, with their log probabilities; 0 <= top <= min(m, 32)
+ *   row_stats[i, 3]  = what euc_label_log_probs_grad needs of the row
+ * log_probs (with labels), entropy and row_stats are nullable.  z = -inf masks a score;
+ * a row with none left has log probabilities of -inf and entropy 0, a row with a NaN or
+ * z = +inf has NaN.  Outputs are fp32 (fp64 for fp64 scores).  scale: finite, not 0. */
+EUC_API int euc_label_log_probs(int row_type, const void* scores, int64_t ld, int64_t n, int64_t m, const void* labels,
+                        int labels_are_i64, double scale, int top, void* log_probs, void* entropy,
+                        void* row_stats, void* top_log_probs, int64_t* top_labels, void* stream);
+/* grad[i, j] (n x m, contiguous, the scores' type) of
+ *   sum_i grad_log_probs[i] log_probs[i] + grad_entropy[i] entropy[i]
+ * with respect to the scores; either gradient is nullable (zero), labels are needed
+ * with grad_log_probs.  A row with no score left has a zero gradient. */
+EUC_API int euc_label_log_probs_grad(int row_type, const void* scores, int64_t ld, int64_t n, int64_t m,
+                             const void* labels, int labels_are_i64, double scale, const void* row_stats,
+                             const void* grad_log_probs, const void* grad_entropy, void* grad, void* stream);
+
+/* The n * p slots (slot i * p + j is label j of row i) sorted by label, stably; labels
+ * outside [0, k) are dropped, as in the center update.
+ *   offsets[c]   (k + 1) first sorted position of label c; offsets[k] = slots kept
+ *   order[r]     slot at sorted position r, -1 for r >= offsets[k]
+ *   position[s]  sorted position of slot s, -1 if dropped
+ *   sorted_labels[r]  label at sorted position r, -1 for r >= offsets[k]
+ * slots and k are at most 2^31 - 2. */
+EUC_API size_t euc_group_rows_workspace_bytes(int64_t slots, int64_t k);
+EUC_API int euc_group_rows(const void* labels, int labels_are_i64, int64_t slots, int64_t k, int32_t* offsets,
+                   int32_t* order, int32_t* position, int32_t* sorted_labels, void* ws, size_t ws_bytes,
+                   void* stream);
+/* Y[position[i, j]] = X[i] (X n x dim, Y n * p x dim); rows of Y behind the last kept
+ * slot are zero.  `kept` is the device address of offsets[k]. */
+EUC_API int euc_rows_to_groups(int row_type, const void* X, const int32_t* position, const int32_t* kept, int64_t n,
+                       int64_t p, int64_t dim, void* Y, void* stream);
+/* out[i] = sum_j weights[i, j] Y[position[i, j]] over the kept slots, in order of j
+ * (weights null: ones); also the gradient of euc_rows_to_groups. */
+EUC_API int euc_rows_from_groups(int row_type, const void* Y, const int32_t* position, const void* weights, int64_t n,
+                         int64_t p, int64_t dim, void* out, void* stream);
+/* Gradients of euc_rows_from_groups: grad_Y[position[i, j]] = weights[i, j] grad_out[i]
+ * (zero rows behind the last kept slot) and, if grad_weights is not null,
+ * grad_weights[i, j] = <grad_out[i], Y[position[i, j]]> (0 where dropped). */
+EUC_API int euc_rows_from_groups_grad(int row_type, const void* grad_out, const void* Y, const int32_t* position,
+                              const void* weights, const int32_t* kept, int64_t n, int64_t p, int64_t dim,
+                              void* grad_Y, void* grad_weights, void* stream);
+
+/* out[i] = scale * C[labels[i]] (C k x dim), a zero row where the label is outside
+ * [0, k); formed in fp32 (fp64 for fp64) and rounded to the type of C. */
+EUC_API int euc_codebook_lookup(int row_type, const void* C, int64_t k, const void* labels, int labels_are_i64,
+                        int64_t n, int64_t dim, double scale, void* out, void* stream);
+/* grad_C[c] = scale * sum of grad_out[i] over the rows with label c (zero without
+ * rows), from the labels' sort (euc_group_rows with p = 1).  Every row of grad_C is
+ * written. */
+EUC_API size_t euc_codebook_grad_workspace_bytes(int row_type, int64_t n, int64_t dim);
+EUC_API int euc_codebook_grad(int row_type, const void* grad_out, const int32_t* offsets, const int32_t* order,
+                      const int32_t* sorted_labels, int64_t n, int64_t k, int64_t dim, double scale, void* grad_C,
+                      void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
