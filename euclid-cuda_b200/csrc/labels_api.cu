@@ -39,10 +39,13 @@ static bool misaligned(int t, std::initializer_list<const void*> ps) {
   return false;
 }
 
-static int scores_shape(int64_t ld, int64_t n, int64_t m, double scale) {
-  if (n < 0 || m < 1 || m > kMaxIndex) return set_error(EUC_ERR_SHAPE, "scores: bad size");
+static int scores_shape(int row_type, int64_t ld, int64_t n, int64_t m, double scale) {
+  if (n < 0 || n > kMaxIndex || m < 1 || m > kMaxIndex) return set_error(EUC_ERR_SHAPE, "scores: bad size");
   if (ld < m && n > 1) return set_error(EUC_ERR_SHAPE, "scores: row stride below the row's length");
   if (!std::isfinite(scale) || scale == 0.0) return set_error(EUC_ERR_ARG, "scale must be finite and not 0");
+  // the fp32 arithmetic holds |scale| and its multiple of log2(e) as normal numbers
+  if (row_type != EUC_ROW_F64 && !(std::fabs(scale) >= 0x1p-126 && std::fabs(scale) <= 0x1p126))
+    return set_error(EUC_ERR_ARG, "scale is outside fp32's range");
   return EUC_OK;
 }
 
@@ -56,7 +59,7 @@ int euc_label_log_probs(int row_type, const void* scores, int64_t ld, int64_t n,
                         int labels_are_i64, double scale, int top, void* log_probs, void* entropy, void* row_stats,
                         void* top_log_probs, int64_t* top_labels, void* stream) {
   if (int rc = bad_type(row_type)) return rc;
-  if (int rc = scores_shape(ld, n, m, scale)) return rc;
+  if (int rc = scores_shape(row_type, ld, n, m, scale)) return rc;
   if (top < 0 || top > kMaxTop || top > m) return set_error(EUC_ERR_UNSUPPORTED, "top must be in [0, min(m, 32)]");
   if (int rc = no_device()) return rc;
   if (n == 0) return EUC_OK;
@@ -85,7 +88,7 @@ int euc_label_log_probs_grad(int row_type, const void* scores, int64_t ld, int64
                              int labels_are_i64, double scale, const void* row_stats, const void* grad_log_probs,
                              const void* grad_entropy, void* grad, void* stream) {
   if (int rc = bad_type(row_type)) return rc;
-  if (int rc = scores_shape(ld, n, m, scale)) return rc;
+  if (int rc = scores_shape(row_type, ld, n, m, scale)) return rc;
   if (int rc = no_device()) return rc;
   if (n == 0) return EUC_OK;
   if (!scores || !row_stats || !grad || (grad_log_probs && !labels)) return set_error(EUC_ERR_ARG, "null pointer");
