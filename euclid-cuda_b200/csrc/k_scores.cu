@@ -32,6 +32,64 @@ __device__ __forceinline__ unsigned long long order_of(double y) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return o == 0xffffffffu ? NAN : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ double value_of(unsigned long long o) {
+  return o == ~0ull ? static_cast<double>(NAN)
+                    : __longlong_as_double(static_cast<long long>(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
+
+// A score and its column, ordered as the alternatives are: y first, equal ones by the lower
+// column.  fp32: one 64-bit number.
+template <typename A> struct Key;
+template <> struct Key<float> {
+  unsigned long long k;
+  __device__ __forceinline__ static Key of(float y, int j) {
+    Key r;
+    r.k = (static_cast<unsigned long long>(order_of(y)) << 32) | (0xffffffffu - static_cast<uint32_t>(j));
+    return r;
+  }
+  __device__ __forceinline__ static Key none() {
+    Key r;
+    r.k = 0;
+    return r;
+  }
+  __device__ __forceinline__ float y() const { return value_of(static_cast<uint32_t>(k >> 32)); }
+  __device__ __forceinline__ int j() const { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+  __device__ __forceinline__ bool ahead(const Key& o) const { return k > o.k; }
+  __device__ __forceinline__ Key other(int s) const {
+    Key r;
+    r.k = __shfl_xor_sync(0xffffffffu, k, s);
+    return r;
+  }
+};
+template <> struct Key<double> {
+  unsigned long long o;
+  long long col;
+  __device__ __forceinline__ static Key of(double y, int j) {
+    Key r;
+    r.o = order_of(y);
+    r.col = j;
+    return r;
+  }
+  __device__ __forceinline__ static Key none() {
+    Key r;
+    r.o = 0;
+    r.col = 0x7fffffff;
+    return r;
+  }
+  __device__ __forceinline__ double y() const { return value_of(o); }
+  __device__ __forceinline__ int j() const { return static_cast<int>(col); }
+  __device__ __forceinline__ bool ahead(const Key& q) const { return o > q.o || (o == q.o && col < q.col); }
+  __device__ __forceinline__ Key other(int s) const {
+    Key r;
+    r.o = __shfl_xor_sync(0xffffffffu, o, s);
+    r.col = __shfl_xor_sync(0xffffffffu, col, s);
+    return r;
+  }
+};
+
 // Exponents are held in units of log 2 for fp32 (t = d log2 e, one ex2 a score; ex2.approx
 // is off by at most 2^-22 of the result and flushes results below 2^-126), in natural units
 // for fp64.  `per_nat` converts mag into a factor of such a unit, `unit` a unit back.
@@ -55,6 +113,10 @@ __device__ __forceinline__ double log_acc(double d) { return log(d); }
 
 template <typename A> __device__ __forceinline__ A neg_inf() { return -static_cast<A>(INFINITY); }
 
+template <typename A> __device__ __forceinline__ A lowest();
+template <> __device__ __forceinline__ float lowest<float>() { return -3.402823466e38f; }
+template <> __device__ __forceinline__ double lowest<double>() { return -1.7976931348623157e308; }
+
 // the larger; NaN if either is
 __device__ __forceinline__ float max_nan(float a, float b) { return fmax_nan(a, b); }
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
@@ -65,11 +127,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 __device__ __forceinline__ double max_nan(double a, double b) { return a != a ? a : (b > a || b != b ? b : a); }
 __device__ __forceinline__ double max_nan(double a, double b, double c) { return max_nan(max_nan(a, b), c); }
 
-template <typename A> __device__ __forceinline__ A warp_sum(A v) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  return v;
-}
 __device__ __forceinline__ float warp_max_nan(float v) {
   float r;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -81,16 +138,19 @@ __device__ __forceinline__ double warp_max_nan(double v) {
   return v;
 }
 
-// The warp's values in descending order over the lanes (bitonic exchanges).
-template <typename A> __device__ __forceinline__ A warp_sort_desc(A v, int lane) {
+// the largest over the TEAM lanes of this lane's team
+template <int TEAM, typename A> __device__ __forceinline__ A team_max_nan(A v) {
+  if constexpr (TEAM == 32) {
+    return warp_max_nan(v);
+  } else {
 #pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
+    for (int s = TEAM / 2; s > 0; s >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, s));
+    return v;
+  }
+}
+template <int TEAM, typename A> __device__ __forceinline__ A team_sum(A v) {
 #pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const A o = __shfl_xor_sync(0xffffffffu, v, j);
-      const bool up = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger
-      v = up ? (o > v ? o : v) : (o < v ? o : v);
-    }
+  for (int s = TEAM / 2; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   return v;
 }
 
@@ -114,12 +174,13 @@ template <typename T> __device__ __forceinline__ int64_t label_of(const void* la
   return i64 ? static_cast<const long long*>(labels)[i] : static_cast<const int*>(labels)[i];
 }
 
-// the row's outputs from its M (as max y), S and T
+// the row's outputs from its M (as max y), S, T, L = log S (-inf for an empty row), and the
+// score at its label (`in`: the label is one of the columns)
 template <typename T>
-__device__ __forceinline__ void write_row(const ScoreArgs<T>& a, int64_t i, Acc<T> hi, Acc<T> S, Acc<T> Tm) {
+__device__ __forceinline__ void write_row(const ScoreArgs<T>& a, int64_t i, Acc<T> hi, Acc<T> S, Acc<T> Tm, Acc<T> L,
+                                          bool in, Acc<T> at_label) {
   using A = Acc<T>;
   const bool empty = hi == neg_inf<A>();
-  const A L = empty ? neg_inf<A>() : log_acc(S);
   const A H = empty ? A(0) : L - Tm / S;
   if (a.entropy) a.entropy[i] = H;
   if (a.stats) {
@@ -127,53 +188,74 @@ __device__ __forceinline__ void write_row(const ScoreArgs<T>& a, int64_t i, Acc<
     a.stats[3 * i + 1] = L;
     a.stats[3 * i + 2] = H;
   }
-  if (a.log_probs) {
-    const int64_t l = label_of<T>(a.labels, a.labels_i64, i);
-    A lp = A(0);
-    if (l >= 0 && l < a.m) lp = empty ? neg_inf<A>() : (a.sign * to_acc(a.x[i * a.ld + l]) - hi) * a.mag - L;
-    a.log_probs[i] = lp;
-  }
-}
-
-template <typename A> struct Best {
-  decltype(order_of(A())) o;
-  int j;
-};
-template <typename A> __device__ __forceinline__ bool before(const Best<A>& p, const Best<A>& q) {
-  return p.o > q.o || (p.o == q.o && p.j < q.j);
+  if (a.log_probs) a.log_probs[i] = !in ? A(0) : empty ? neg_inf<A>() : (at_label - hi) * a.mag - L;
 }
 
 // ------------------------------------------------------------------ a row as vectors
+// the elements of 16 bytes
+template <typename T> __device__ __forceinline__ void unpack(const uint4& w, Acc<T>* y) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      y[2 * q] = __uint_as_float(r[q] << 16);
+      y[2 * q + 1] = __uint_as_float(r[q] & 0xffff0000u);
+    }
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[q]));
+      y[2 * q] = f.x;
+      y[2 * q + 1] = f.y;
+    }
+  } else {
+    Vec<T, 16 / static_cast<int>(sizeof(T))> v;
+    v.raw = w;
+#pragma unroll
+    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) y[e] = v.e[e];
+  }
+}
+
 // Vector v of a row is the 16 bytes at its v-th 16-byte boundary, counted from the one at or
-// before the row's start (`off` elements before it).  Elements outside the row read as -inf
-// in y, which adds nothing to any sum; nothing outside the row is read.
+// before the row's start (`off` elements before it): [0, all) of them, of which [lo, hi) lie
+// in the row whole.  The others are read element by element; nothing outside the row is read.
+// y = -x where the scale is negative: the sign bits are flipped in the 16 bytes.
 template <typename T> struct RowVecs {
   static constexpr int VE = 16 / static_cast<int>(sizeof(T));
   const T* x;
-  int m, off;
-  __device__ __forceinline__ RowVecs(const T* x_, int m_) : x(x_), m(m_) {
+  const uint4* base;
+  int m, off, all, lo, hi;
+  uint32_t flip_even, flip_odd;  // of the words 0, 2 and 1, 3
+  __device__ __forceinline__ RowVecs(const T* x_, int m_, bool negate) : x(x_), m(m_) {
     off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    base = reinterpret_cast<const uint4*>(x - off);
+    all = (m + off + VE - 1) / VE;
+    lo = off > 0 ? 1 : 0;
+    hi = (m + off) / VE;
+    const uint32_t odd = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+    flip_odd = negate ? odd : 0u;
+    flip_even = sizeof(T) == 8 ? 0u : flip_odd;
   }
-  __device__ __forceinline__ int64_t count() const { return (static_cast<int64_t>(m) + off + VE - 1) / VE; }
-  __device__ __forceinline__ int64_t first(int64_t v) const { return v * VE - off; }
-  // the 16 bytes; `negate` flips the signs (y = -x)
-  __device__ __forceinline__ void load(int64_t v, bool negate, Acc<T>* y) const {
-    const int64_t j = first(v);
-    Vec<T, VE> w;
-    if (j >= 0 && j + VE <= m) {
-      w.raw = load_keep(reinterpret_cast<const uint4*>(x + j));
+  __device__ __forceinline__ uint4 read(int v) const { return load_keep(base + v); }
+  __device__ __forceinline__ void values(uint4 w, Acc<T>* y) const {
+    w.x ^= flip_even;
+    w.y ^= flip_odd;
+    w.z ^= flip_even;
+    w.w ^= flip_odd;
+    unpack<T>(w, y);
+  }
+  __device__ __forceinline__ Acc<T> at(int j) const { return flip_odd ? -to_acc(x[j]) : to_acc(x[j]); }
+  // any vector of [0, all); elements outside the row are -inf
+  __device__ __forceinline__ void load(int v, Acc<T>* y) const {
+    if (v >= lo && v < hi) {
+      values(read(v), y);
+      return;
+    }
 #pragma unroll
-      for (int e = 0; e < VE; ++e) y[e] = to_acc(w.e[e]);
-      if (negate) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) y[e] = -y[e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        y[e] = neg_inf<Acc<T>>();
-        if (j + e >= 0 && j + e < m) y[e] = negate ? -to_acc(x[j + e]) : to_acc(x[j + e]);
-      }
+    for (int e = 0; e < VE; ++e) {
+      const int j = v * VE - off + e;
+      y[e] = j >= 0 && j < m ? at(j) : neg_inf<Acc<T>>();
     }
   }
 };
@@ -248,123 +330,185 @@ __device__ __forceinline__ void both(const Sums<double>& p, double& s, double& t
 }
 
 // ------------------------------------------------------------------ the alternatives
-// The `top` best of a row without sorting it: any number t that at least `top` scores reach
-// bounds the last of them from below, and few scores reach a good one.  t comes from the
-// lanes' maxima, which the softmax needs anyhow; the scores that reach it go to a list in
-// shared memory (in any order), and a candidate's place is the number of candidates before
-// it.  More candidates than the list holds (many equal scores), or a NaN, take the plain way:
-// the best one behind the last one, `top` times.
-template <typename A> struct Cand {
-  A y;
-  int j;
-};
-template <typename A> __device__ __forceinline__ bool ahead(const Cand<A>& p, const Cand<A>& q) {
-  return p.y > q.y || (p.y == q.y && p.j < q.j);
+// The `top` best of a row without sorting it: any number that at least `top` scores reach
+// bounds the last of them from below, and few scores reach a good one.  The bound comes from
+// maxima that the softmax needs anyhow: the row is cut into lists of maxima (over the lanes),
+// and with q = ceil(top / lists) the smallest of the lists' q-th largest is reached by q of
+// every list.  The scores that reach it go to a candidate list in shared memory (in any
+// order), and a candidate's place is the number of candidates before it.  More candidates
+// than the list holds (many equal scores), or a NaN, take the plain way: the best one behind
+// the last one, `top` times.
+// The q-th largest over the team's lanes of each list, the smallest over the lists: q - 1
+// rounds strike each list's largest (and its equals, which only lowers the bound).  No NaN.
+// A row that is masked but for fewer scores gives the lowest finite number.
+template <int TEAM, int LISTS, typename A> __device__ __forceinline__ A team_bound(A* lists, int q) {
+  A t[LISTS];
+#pragma unroll
+  for (int l = 0; l < LISTS; ++l) t[l] = team_max_nan<TEAM>(lists[l]);
+  for (int k = 1; k < q; ++k) {
+#pragma unroll
+    for (int l = 0; l < LISTS; ++l) lists[l] = lists[l] == t[l] ? neg_inf<A>() : lists[l];
+#pragma unroll
+    for (int l = 0; l < LISTS; ++l) t[l] = team_max_nan<TEAM>(lists[l]);
+  }
+#pragma unroll
+  for (int l = 1; l < LISTS; ++l) t[0] = t[l] < t[0] ? t[l] : t[0];
+  return t[0] > lowest<A>() ? t[0] : lowest<A>();
 }
 
 template <typename T>
-__device__ __forceinline__ void write_top(const ScoreArgs<T>& a, int64_t i, int place, Acc<T> y, int j, Acc<T> hi,
+__device__ __forceinline__ void write_top(const ScoreArgs<T>& a, int64_t i, int place, const Key<Acc<T>>& k, Acc<T> hi,
                                           Acc<T> L) {
-  a.top_labels[i * a.top + place] = j;
-  a.top_log_probs[i * a.top + place] = hi == neg_inf<Acc<T>>() ? hi : (y - hi) * a.mag - L;
+  a.top_labels[i * a.top + place] = k.j();
+  a.top_log_probs[i * a.top + place] = hi == neg_inf<Acc<T>>() ? hi : (k.y() - hi) * a.mag - L;
 }
 
-// ------------------------------------------------------------------ one warp per row
-// Rows of up to 32 EPL scores: the row stays in registers, so its scores are read once and
-// its maximum is known before the first exponential.
-constexpr int kWarpCands = 128;
+// how many of list[0, count) are ahead of `me`
+template <typename A> __device__ __forceinline__ int place_of(const Key<A>* list, int count, const Key<A>& me) {
+  int place = 0;
+#pragma unroll 4
+  for (int r = 0; r < count; ++r) place += list[r].ahead(me) ? 1 : 0;
+  return place;
+}
 
-template <typename T, int EPL>
-__global__ void __launch_bounds__(128) scores_warp_kernel(ScoreArgs<T> a) {
+// ------------------------------------------------------------------ a team of lanes per row
+// Rows of up to TEAM EPL scores, a team of 8 or 32 lanes each: the row stays in registers, so
+// its scores are read once and its maximum is known before the first exponential; a warp
+// reads its next rows while it works on these (not with 64 scores a lane, whose registers
+// are better spent on more warps).  FLAT: every row is whole 16-byte vectors;
+// other rows are read element by element, neighbouring lanes neighbouring elements.
+constexpr int kTeamCands = 256;  // per warp
+
+template <typename T, int TEAM, int EPL, bool FLAT>
+__global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) >= 256 ? (sizeof(T) == 8 ? 2 : 4) : 5) scores_team_kernel(ScoreArgs<T> a) {
   using A = Acc<T>;
-  constexpr int VE = RowVecs<T>::VE, NV = EPL / VE;
-  __shared__ Cand<A> cands[4][kWarpCands];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int VE = FLAT ? RowVecs<T>::VE : 1, NV = EPL / VE, RPW = 32 / TEAM, CAP = kTeamCands / RPW;
+  constexpr bool AHEAD = EPL <= 32;
+  __shared__ Key<A> cands[4][kTeamCands];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tl = lane % TEAM, team = lane / TEAM;
+  const unsigned team_lanes = (TEAM == 32 ? 0xffffffffu : (1u << (TEAM & 31)) - 1u) << (team * TEAM);
+  const unsigned before_me = team_lanes & ((1u << lane) - 1u);
   const bool negate = a.sign < A(0);
   const A c = a.mag * Expo<A>::per_nat;
-  Cand<A>* list = cands[warp];
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + warp; i < a.n; i += static_cast<int64_t>(gridDim.x) * 4) {
-    const RowVecs<T> row(a.x + i * a.ld, a.m);
+  Key<A>* list = cands[warp] + team * CAP;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (4 * RPW);
+  int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + warp) * RPW;
+  if (first >= a.n) return;
+  using Raw = typename std::conditional<FLAT, uint4, T>::type;
+  Raw next[NV];
+  int64_t next_label = -1;
+  // vectors behind the row's end hold z = -inf from the start, and no load changes them
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    Vec<T, FLAT ? VE : 1> fill;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) fill.e[e] = from_acc<T>(negate ? -neg_inf<A>() : neg_inf<A>());
+    if constexpr (FLAT) next[v] = fill.raw;
+    else next[v] = fill.e[0];
+  }
+  auto fetch = [&](int64_t row) {
+    row = min(row, a.n - 1);
+    const T* x = a.x + row * a.ld;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if ((v * TEAM + tl) * VE < a.m) next[v] = load_keep(reinterpret_cast<const Raw*>(x) + v * TEAM + tl);
+    if (a.log_probs) next_label = label_of<T>(a.labels, a.labels_i64, row);
+  };
+  if (AHEAD) fetch(first + team);
+  for (; first < a.n; first += step) {
+    if (!AHEAD) fetch(first + team);
+    const bool live = first + team < a.n;
+    const int64_t i = live ? first + team : a.n - 1;
+    const RowVecs<T> row(a.x + i * a.ld, a.m, negate);
     A y[EPL];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) row.load(v * 32 + lane, negate, y + v * VE);
-    const A mine = max_of<A, EPL>(y);
-    const A hi = warp_max_nan(mine);
+    for (int v = 0; v < NV; ++v) {
+      if constexpr (FLAT) row.values(next[v], y + v * VE);
+      else y[v] = negate ? -to_acc(next[v]) : to_acc(next[v]);
+    }
+    const bool labelled = next_label >= 0 && next_label < a.m;
+    const A at_label = labelled ? row.at(static_cast<int>(next_label)) : A(0);  // ready by the time it is needed
+    if (AHEAD && first + step < a.n) fetch(first + step + team);
+    A lists[4];
+#pragma unroll
+    for (int l = 0; l < 4; ++l) lists[l] = max_of<A, EPL / 4>(y + l * (EPL / 4));
+    const A hi = team_max_nan<TEAM>(max_nan(max_nan(lists[0], lists[1]), lists[2], lists[3]));
     Sums<A> sums;
     sums.template add<EPL>(y, hi == neg_inf<A>() ? A(0) : hi, c);
     A S, Tm;
     both(sums, S, Tm);
-    S = warp_sum(S);
-    Tm = warp_sum(Tm) * Expo<A>::unit;
-    const bool odd = hi != hi || hi == -neg_inf<A>();
-    if (odd) S = Tm = static_cast<A>(NAN);
-    if (lane == 0) write_row(a, i, hi, S, Tm);
-    if (a.top == 0) continue;
+    S = team_sum<TEAM>(S);
+    Tm = team_sum<TEAM>(Tm) * Expo<A>::unit;
+    if (hi != hi || hi == -neg_inf<A>()) S = Tm = static_cast<A>(NAN);
     const A L = hi == neg_inf<A>() ? hi : log_acc(S);
+    if (tl == 0 && live) write_row(a, i, hi, S, Tm, L, labelled, at_label);
+    if (a.top == 0) continue;
     bool slow = hi != hi;
     int count = 0;
-    if (!slow) {
-      const A t = __shfl_sync(0xffffffffu, warp_sort_desc(mine, lane), a.top - 1);
-      const bool none = t == neg_inf<A>();  // fewer than `top` lanes hold a score
-#pragma unroll
-      for (int q = 0; q < EPL; ++q) {
-        const bool in = none ? y[q] > t : y[q] >= t;
-        const unsigned b = __ballot_sync(0xffffffffu, in);
-        if (b == 0u) continue;
-        const int at = count + __popc(b & ((1u << lane) - 1u));
-        if (in && at < kWarpCands) {
-          list[at].y = y[q];
-          list[at].j = static_cast<int>(row.first((q / VE) * 32 + lane)) + q % VE;
-        }
-        count += __popc(b);
-      }
-      if (none) {  // masked scores by index: the first 2 top hold enough of them
-        for (int j0 = 0; j0 < min(a.m, 2 * a.top); j0 += 32) {
-          const int j = j0 + lane;
-          const bool in = j < min(a.m, 2 * a.top) && a.sign * to_acc(row.x[j]) == neg_inf<A>();
-          const unsigned b = __ballot_sync(0xffffffffu, in);
-          const int at = count + __popc(b & ((1u << lane) - 1u));
-          if (in && at < kWarpCands) {
-            list[at].y = neg_inf<A>();
-            list[at].j = j;
-          }
-          count += __popc(b);
-        }
-      }
-      slow = count > kWarpCands;
-    }
-    __syncwarp();
-    if (!slow) {
-      for (int q = lane; q < count; q += 32) {
-        const Cand<A> me = list[q];
-        int place = 0;
-        for (int r = 0; r < count; ++r) place += ahead(list[r], me) ? 1 : 0;
-        if (place < a.top) write_top(a, i, place, me.y, me.j, hi, L);
-      }
+    // fewer lists give a better bound, more of them fewer rounds
+    A t;
+    if (a.top <= 4) {
+      lists[0] = max_nan(max_nan(lists[0], lists[1]), lists[2], lists[3]);
+      t = team_bound<TEAM, 1>(lists, a.top);
+    } else if (a.top <= 16) {
+      lists[0] = max_nan(lists[0], lists[1]);
+      lists[1] = max_nan(lists[2], lists[3]);
+      t = team_bound<TEAM, 2>(lists, (a.top + 1) / 2);
     } else {
-      Best<A> last{};
-      for (int k = 0; k < a.top; ++k) {
-        Best<A> best;
-        best.o = 0;
-        best.j = 0x7fffffff;
+      t = team_bound<TEAM, 4>(lists, (a.top + 3) / 4);
+    }
 #pragma unroll
-        for (int q = 0; q < EPL; ++q) {
-          const int64_t j = row.first((q / VE) * 32 + lane) + q % VE;
-          if (j < 0 || j >= a.m) continue;
-          Best<A> o;
-          o.o = order_of(y[q]);
-          o.j = static_cast<int>(j);
-          if ((k == 0 || before(last, o)) && before(o, best)) best = o;
+    for (int w = 0; w < EPL; w += 32) {
+      uint32_t in = 0u;
+#pragma unroll
+      for (int q = 0; q < (EPL < 32 ? EPL : 32); ++q) in |= y[w + q] >= t ? 1u << q : 0u;
+      while (true) {
+        const unsigned b = __ballot_sync(0xffffffffu, in != 0u);
+        if (b == 0u) break;
+        if (in != 0u) {
+          const int at = count + __popc(b & before_me), q = w + __ffs(in) - 1;
+          const int j = ((q / VE) * TEAM + tl) * VE + q % VE;
+          if (at < CAP) list[at] = Key<A>::of(row.at(j), j);
+          in &= in - 1u;
+        }
+        count += __popc(b & team_lanes);
+      }
+    }
+    if (__any_sync(0xffffffffu, t == lowest<A>())) {
+      // masked scores by index: the first 2 top hold enough of them
+      for (int j0 = 0; j0 < min(a.m, 2 * a.top); j0 += TEAM) {
+        const int j = j0 + tl;
+        const bool here = t == lowest<A>() && j < min(a.m, 2 * a.top) && row.at(j) == neg_inf<A>();
+        const unsigned b = __ballot_sync(0xffffffffu, here);
+        const int at = count + __popc(b & before_me);
+        if (here && at < CAP) list[at] = Key<A>::of(neg_inf<A>(), j);
+        count += __popc(b & team_lanes);
+      }
+    }
+    slow |= count > CAP;
+    __syncwarp();
+    if (!slow && live) {
+      for (int q = tl; q < count; q += TEAM) {
+        const Key<A> me = list[q];
+        const int place = place_of(list, count, me);
+        if (place < a.top) write_top(a, i, place, me, hi, L);
+      }
+    }
+    if (__any_sync(0xffffffffu, slow)) {
+      Key<A> last = Key<A>::none();
+      for (int k = 0; k < a.top; ++k) {
+        Key<A> best = Key<A>::none();
+        for (int j = tl; j < a.m; j += TEAM) {
+          const Key<A> o = Key<A>::of(row.at(j), j);
+          if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
         }
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-          Best<A> o;
-          o.o = __shfl_xor_sync(0xffffffffu, best.o, s);
-          o.j = __shfl_xor_sync(0xffffffffu, best.j, s);
-          if (before(o, best)) best = o;
+        for (int s = TEAM / 2; s > 0; s >>= 1) {
+          const Key<A> o = best.other(s);
+          if (o.ahead(best)) best = o;
         }
         last = best;
-        if (lane == 0) write_top(a, i, k, a.sign * to_acc(row.x[best.j]), best.j, hi, L);
+        if (tl == 0 && slow && live) write_top(a, i, k, best, hi, L);
       }
     }
     __syncwarp();
@@ -391,6 +535,7 @@ template <typename V> __device__ __forceinline__ void store_cluster(const V* at,
 constexpr int kGroups = 32;       // groups of vectors per thread
 constexpr int kBlockVecs = 4;     // vectors in flight per thread
 constexpr int kBlockCands = 512;
+constexpr int kBlockHits = 256;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 
@@ -400,49 +545,98 @@ template <typename A> struct Part {  // one block's share of a row
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int cluster, int per_group) {
+__global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int log_cluster, int per_group) {
   using A = Acc<T>;
-  constexpr int VE = RowVecs<T>::VE, U = kBlockVecs, W = NT / 32;
+  constexpr int VE = RowVecs<T>::VE, U = kBlockVecs, W = NT / 32, LISTS = W == 1 ? U : 1;
   extern __shared__ __align__(16) unsigned char dyn[];
   A* group_max = reinterpret_cast<A*>(dyn);  // [kGroups][NT], with alternatives only
-  __shared__ Cand<A> cands[kBlockCands];
-  __shared__ Cand<A> lists[kMaxCluster][kMaxTop];
+  __shared__ Key<A> cands[kBlockCands];
+  __shared__ uint32_t hits[kBlockHits];  // (group of vectors, thread) with a score that reaches the bound
+  __shared__ Key<A> lists[kMaxCluster][kMaxTop];
   __shared__ Part<A> parts[kMaxCluster];
-  __shared__ A red[3][W];
-  __shared__ int count_sh;
+  __shared__ A red[2][W];
+  __shared__ int count_sh, hits_sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t i = blockIdx.x / cluster;
-  const int rank = static_cast<int>(blockIdx.x - i * cluster);
-  const bool negate = a.sign < A(0);
+  const int cluster = 1 << log_cluster;
+  const int64_t i = blockIdx.x >> log_cluster;
+  const int rank = static_cast<int>(blockIdx.x) & (cluster - 1);
   const A c = a.mag * Expo<A>::per_nat;
-  const RowVecs<T> row(a.x + i * a.ld, a.m);
-  const int64_t all = row.count(), per = (all + cluster - 1) / cluster;
-  const int64_t v0 = min(all, rank * per), v1 = min(all, v0 + per);
-  const int steps = static_cast<int>((v1 - v0 + U * NT - 1) / (U * NT));
-  if (threadIdx.x == 0) count_sh = 0;
+  const RowVecs<T> row(a.x + i * a.ld, a.m, a.sign < A(0));
+  const int per = (row.all + cluster - 1) >> log_cluster;
+  const int v0 = min(row.all, rank * per), v1 = min(row.all, v0 + per);
+  const int j0 = max(0, v0 * VE - row.off), j1 = max(j0, min(a.m, v1 * VE - row.off));  // the slice's scores
+  const int i0 = max(v0, row.lo), i1 = max(i0, min(v1, row.hi));                        // its whole vectors
+  const int steps = (i1 - i0 + U * NT - 1) / (U * NT);
+  // the first and the last vector where they are not whole: the first and the last thread
+  int edge = -1;
+  if (threadIdx.x == 0 && row.lo > 0 && v0 == 0) edge = 0;
+  if (threadIdx.x == NT - 1 && row.hi < row.all && v1 == row.all && v0 < v1 && !(row.lo > 0 && row.all == 1)) edge = row.all - 1;
+  if (threadIdx.x == 0) count_sh = hits_sh = 0;
   if (cluster > 1) cluster_arrive();  // waited for before the first store to another block
 
-  A mine = neg_inf<A>(), gm = neg_inf<A>();
+  // the label's score, read ahead of its use
+  bool labelled = false;
+  A at_label = A(0);
+  if (rank == 0 && threadIdx.x == 0 && a.log_probs) {
+    const int64_t l = label_of<T>(a.labels, a.labels_i64, i);
+    labelled = l >= 0 && l < a.m;
+    if (labelled) at_label = row.at(static_cast<int>(l));
+  }
+
+  A mine = neg_inf<A>(), gm = neg_inf<A>(), edge_max = neg_inf<A>();
+  A slot_max[LISTS];  // of one warp's lists: a maximum per vector in flight
+#pragma unroll
+  for (int l = 0; l < LISTS; ++l) slot_max[l] = neg_inf<A>();
   Sums<A> sums;
-  int g = 0, in_group = 0;
-  for (int s = 0; s < steps; ++s) {
-    A y[U * VE];
-    const int64_t v = v0 + static_cast<int64_t>(s) * (U * NT) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v + u * NT < v1) {
-        row.load(v + u * NT, negate, y + u * VE);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) y[u * VE + e] = neg_inf<A>();
-      }
-    }
-    const A most = max_of<A, U * VE>(y);
-    gm = max_nan(gm, most);
-    if (!(most <= mine)) {  // larger, or a NaN
+  auto take = [&](A most) {  // a new maximum of the thread: larger, or a NaN
+    if (!(most <= mine)) {
       if (mine > neg_inf<A>()) sums.move((mine - most) * c);
       mine = max_nan(mine, most);
     }
+  };
+  if (edge >= 0) {
+    A y[VE];
+    row.load(edge, y);
+    edge_max = max_of<A, VE>(y);
+    take(edge_max);
+    sums.template add<VE>(y, mine == neg_inf<A>() ? A(0) : mine, c);
+  }
+  int g = 0, in_group = 0;
+  const uint4* from = row.base + i0 + threadIdx.x;
+  for (int s = 0; s < steps; ++s, from += U * NT) {
+    A y[U * VE];
+    if ((s + 1) * (U * NT) <= i1 - i0) {
+      uint4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = load_keep(from + u * NT);
+#pragma unroll
+      for (int u = 0; u < U; ++u) row.values(w[u], y + u * VE);
+    } else {
+      const int left = i1 - i0 - s * (U * NT) - static_cast<int>(threadIdx.x);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u * NT < left) {
+          row.values(load_keep(from + u * NT), y + u * VE);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) y[u * VE + e] = neg_inf<A>();
+        }
+      }
+    }
+    A most;
+    if constexpr (LISTS > 1) {
+      A m4[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        m4[u] = max_of<A, VE>(y + u * VE);
+        slot_max[u] = max_nan(slot_max[u], m4[u]);
+      }
+      most = max_of<A, U>(m4);
+    } else {
+      most = max_of<A, U * VE>(y);
+    }
+    gm = max_nan(gm, most);
+    take(most);
     sums.template add<U * VE>(y, mine == neg_inf<A>() ? A(0) : mine, c);
     if (++in_group == per_group) {
       if (a.top) group_max[g * NT + threadIdx.x] = gm;
@@ -455,35 +649,33 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int cl
 
   // the block's maximum and sums, and the alternatives' bound
   const A wmax = warp_max_nan(mine);
-  const int want = static_cast<int>(min(static_cast<int64_t>(a.top), (v1 - v0) * VE));
-  A some = neg_inf<A>(), each = neg_inf<A>();
-  if (a.top && want > 0) {
-    // `want` scores reach the warp's want-th largest lane maximum; ceil(want / W) in every
-    // warp reach the smallest of the warps' ceil(want / W)-th largest
-    const A sorted = warp_sort_desc(mine, lane);
-    some = __shfl_sync(0xffffffffu, sorted, want - 1);
-    each = __shfl_sync(0xffffffffu, sorted, (want + W - 1) / W - 1);
+  const int want = min(a.top, j1 - j0);
+  A bound = lowest<A>();
+  if (want > 0) {
+    constexpr int ALL = W * LISTS;
+    if constexpr (LISTS == 1) slot_max[0] = mine;
+    else slot_max[0] = max_nan(slot_max[0], edge_max);
+    bound = team_bound<32, LISTS>(slot_max, (want + ALL - 1) / ALL);
   }
   if (lane == 0) {
     red[0][warp] = wmax;
-    red[1][warp] = some;
-    red[2][warp] = each;
+    red[1][warp] = bound;
   }
   __syncthreads();
-  A hi = red[0][0], bound = red[1][0], least = red[2][0];
+  A hi = red[0][0];
+  bound = red[1][0];
 #pragma unroll
   for (int w = 1; w < W; ++w) {
     hi = max_nan(hi, red[0][w]);
-    bound = red[1][w] > bound ? red[1][w] : bound;
-    least = red[2][w] < least ? red[2][w] : least;
+    bound = red[1][w] < bound ? red[1][w] : bound;
   }
-  bound = least > bound ? least : bound;
+  if (want == 1 && hi > bound) bound = hi;
   __syncthreads();
   if (mine > neg_inf<A>()) sums.move((mine - hi) * c);
   A S, Tm;
   both(sums, S, Tm);
-  S = warp_sum(S);
-  Tm = warp_sum(Tm);
+  S = team_sum<32>(S);
+  Tm = team_sum<32>(Tm);
   if (lane == 0) {
     red[0][warp] = S;
     red[1][warp] = Tm;
@@ -496,164 +688,126 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int cl
     Tm += red[1][w];
   }
 
-  // this block's best `want` scores, in order, in list[rank]
-  Cand<A>* list = lists[rank];
-  const bool has_nan = hi != hi;
-  if (a.top && want > 0) {
-    const bool none = bound == neg_inf<A>();
-    bool slow = has_nan;
+  // this block's best `want` scores, in order, in lists[rank]
+  Key<A>* list = lists[rank];
+  if (want > 0) {
+    bool slow = hi != hi;
     if (!slow) {
-      for (int q = 0; q * per_group < steps; ++q) {
-        const A top_of = group_max[q * NT + threadIdx.x];
-        if (none ? !(top_of > bound) : !(top_of >= bound)) continue;
-        for (int s = q * per_group; s < min(steps, (q + 1) * per_group); ++s)
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int64_t v = v0 + static_cast<int64_t>(s) * (U * NT) + u * NT + threadIdx.x;
-            if (v >= v1) continue;
-            A y[VE];
-            row.load(v, negate, y);
-#pragma unroll
-            for (int e = 0; e < VE; ++e)
-              if (none ? y[e] > bound : y[e] >= bound) {
-                const int at = atomicAdd(&count_sh, 1);
-                if (at < kBlockCands) {
-                  cands[at].y = y[e];
-                  cands[at].j = static_cast<int>(row.first(v)) + e;
-                }
-              }
+      auto add = [&](A y, int j) {
+        const int at = atomicAdd(&count_sh, 1);
+        if (at < kBlockCands) cands[at] = Key<A>::of(y, j);
+      };
+      if (mine >= bound)
+        for (int q = 0; q * per_group < steps; ++q)
+          if (group_max[q * NT + threadIdx.x] >= bound) {
+            const int at = atomicAdd(&hits_sh, 1);
+            if (at < kBlockHits) hits[at] = static_cast<uint32_t>(q) * NT + threadIdx.x;
           }
-      }
-      if (none) {  // masked scores by index, from the slice's first 2 want
-        const int64_t j = max(static_cast<int64_t>(0), row.first(v0)) + threadIdx.x;
-        if (threadIdx.x < 2 * want && j < a.m && j < row.first(v1) && a.sign * to_acc(row.x[j]) == neg_inf<A>()) {
-          const int at = atomicAdd(&count_sh, 1);
-          if (at < kBlockCands) {
-            cands[at].y = neg_inf<A>();
-            cands[at].j = static_cast<int>(j);
+      if (edge >= 0 && edge_max >= bound)
+        for (int e = 0; e < VE; ++e) {
+          const int j = edge * VE - row.off + e;
+          if (j >= 0 && j < a.m && row.at(j) >= bound) add(row.at(j), j);
+        }
+      if (bound == lowest<A>())  // masked scores by index, from the slice's first 2 want
+        for (int j = j0 + static_cast<int>(threadIdx.x); j < min(j1, j0 + 2 * want); j += NT)
+          if (row.at(j) == neg_inf<A>()) add(neg_inf<A>(), j);
+      __syncthreads();
+      slow = hits_sh > kBlockHits;
+      if (!slow) {  // a warp per group of vectors, a lane per score
+        const int found = hits_sh;
+        for (int h = warp; h < found; h += W) {
+          const int q = static_cast<int>(hits[h] / NT), thread = static_cast<int>(hits[h] % NT);
+          for (int z = lane; z < per_group * (U * VE); z += 32) {
+            const int s = q * per_group + z / (U * VE), u = z / VE % U;
+            const int v = i0 + s * (U * NT) + u * NT + thread;
+            if (v >= i1) continue;
+            const int j = v * VE - row.off + z % VE;
+            const A y = row.at(j);
+            if (y >= bound) add(y, j);
           }
         }
       }
       __syncthreads();
-      slow = count_sh > kBlockCands;
+      slow |= count_sh > kBlockCands;
     }
     if (!slow) {
       const int count = count_sh;
       for (int q = threadIdx.x; q < count; q += NT) {
-        const Cand<A> me = cands[q];
-        int place = 0;
-        for (int r = 0; r < count; ++r) place += ahead(cands[r], me) ? 1 : 0;
+        const Key<A> me = cands[q];
+        const int place = place_of(cands, count, me);
         if (place < want) list[place] = me;
       }
-      if (threadIdx.x == 0) parts[rank].count = min(count, want);
     } else {
-      Best<A>* redb = reinterpret_cast<Best<A>*>(cands);
-      Best<A> last{};
-      int k = 0;
-      for (; k < want; ++k) {
-        Best<A> best;
-        best.o = 0;
-        best.j = 0x7fffffff;
-        for (int64_t v = v0 + threadIdx.x; v < v1; v += NT) {
-          A y[VE];
-          row.load(v, negate, y);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const int64_t j = row.first(v) + e;
-            if (j < 0 || j >= a.m) continue;
-            Best<A> o;
-            o.o = order_of(y[e]);
-            o.j = static_cast<int>(j);
-            if ((k == 0 || before(last, o)) && before(o, best)) best = o;
-          }
+      Key<A> last = Key<A>::none();
+      for (int k = 0; k < want; ++k) {
+        Key<A> best = Key<A>::none();
+        for (int j = j0 + static_cast<int>(threadIdx.x); j < j1; j += NT) {
+          const Key<A> o = Key<A>::of(row.at(j), j);
+          if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
         }
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) {
-          Best<A> o;
-          o.o = __shfl_xor_sync(0xffffffffu, best.o, s);
-          o.j = __shfl_xor_sync(0xffffffffu, best.j, s);
-          if (before(o, best)) best = o;
+          const Key<A> o = best.other(s);
+          if (o.ahead(best)) best = o;
         }
         __syncthreads();
-        if (lane == 0) redb[warp] = best;
+        if (lane == 0) cands[warp] = best;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w)
-          if (before(redb[w], best)) best = redb[w];
-        if (best.j == 0x7fffffff) break;  // the slice is shorter than `want`
+          if (cands[w].ahead(best)) best = cands[w];
         last = best;
-        if (threadIdx.x == 0) {
-          list[k].y = a.sign * to_acc(row.x[best.j]);
-          list[k].j = best.j;
-        }
+        if (threadIdx.x == 0) list[k] = best;
       }
-      if (threadIdx.x == 0) parts[rank].count = k;
     }
-  } else if (threadIdx.x == 0) {
-    parts[rank].count = 0;
   }
-  if (threadIdx.x == 0) {
-    parts[rank].hi = hi;
-    parts[rank].S = S;
-    parts[rank].T = Tm;
-  }
-  __syncthreads();
   if (cluster > 1) {
+    if (threadIdx.x == 0) {
+      parts[rank].hi = hi;
+      parts[rank].S = S;
+      parts[rank].T = Tm;
+      parts[rank].count = want;
+    }
+    __syncthreads();
     cluster_wait();
     if (rank > 0) {
       if (threadIdx.x == 0) store_cluster(&parts[rank], parts[rank]);
-      for (int q = threadIdx.x; q < parts[rank].count; q += NT) store_cluster(&list[q], list[q]);
+      for (int q = threadIdx.x; q < want; q += NT) store_cluster(&list[q], list[q]);
     }
     __syncthreads();
     cluster_sync();
     if (rank > 0) return;
-  }
-
-  // the row's results, by the first block
-  bool any_nan = false;
-  hi = neg_inf<A>();
-  for (int r = 0; r < cluster; ++r) {
-    any_nan |= parts[r].hi != parts[r].hi;
-    hi = max_nan(hi, parts[r].hi);
-  }
-  S = Tm = A(0);
-  for (int r = 0; r < cluster; ++r) {
-    if (!(parts[r].hi > neg_inf<A>())) continue;
-    const A drop = (parts[r].hi - hi) * c;
-    const bool far = !(drop > Expo<A>::floor);
-    const A f = far ? A(0) : Expo<A>::exp(drop);
-    S += f * parts[r].S;
-    Tm += f * (parts[r].T + parts[r].S * (far ? A(0) : drop));
+    // the row's results, by the first block
+    hi = neg_inf<A>();
+    for (int r = 0; r < cluster; ++r) hi = max_nan(hi, parts[r].hi);
+    S = Tm = A(0);
+    for (int r = 0; r < cluster; ++r) {
+      if (!(parts[r].hi > neg_inf<A>())) continue;
+      const A drop = (parts[r].hi - hi) * c;
+      const bool far = !(drop > Expo<A>::floor);
+      const A f = far ? A(0) : Expo<A>::exp(drop);
+      S += f * parts[r].S;
+      Tm += f * (parts[r].T + parts[r].S * (far ? A(0) : drop));
+    }
+  } else {
+    __syncthreads();
   }
   Tm *= Expo<A>::unit;
-  if (any_nan || hi == -neg_inf<A>()) S = Tm = static_cast<A>(NAN);
-  if (threadIdx.x == 0) write_row(a, i, hi, S, Tm);
-  if (!a.top) return;
+  if (hi != hi || hi == -neg_inf<A>()) S = Tm = static_cast<A>(NAN);
   const A L = hi == neg_inf<A>() ? hi : log_acc(S);
-  for (int q = threadIdx.x; q < cluster * a.top; q += NT) {
-    const int r = q / a.top, k = q - r * a.top;
+  if (threadIdx.x == 0) write_row(a, i, hi, S, Tm, L, labelled, at_label);
+  if (cluster == 1) {
+    if (static_cast<int>(threadIdx.x) < a.top) write_top(a, i, static_cast<int>(threadIdx.x), list[threadIdx.x], hi, L);
+    return;
+  }
+  for (int q = threadIdx.x; q < cluster * kMaxTop; q += NT) {
+    const int r = q / kMaxTop, k = q % kMaxTop;
     if (k >= parts[r].count) continue;
-    const Cand<A> me = lists[r][k];
+    const Key<A> me = lists[r][k];
     int place = k;  // the lists are in order: only the others' candidates are counted
-    for (int o = 0; o < cluster; ++o) {
-      if (o == r) continue;
-      for (int z = 0; z < parts[o].count; ++z) {
-        const Cand<A> he = lists[o][z];
-        bool first;
-        if (any_nan) {
-          Best<A> p, w;
-          p.o = order_of(he.y);
-          p.j = he.j;
-          w.o = order_of(me.y);
-          w.j = me.j;
-          first = before(p, w);
-        } else {
-          first = ahead(he, me);
-        }
-        place += first ? 1 : 0;
-      }
-    }
-    if (place < a.top) write_top(a, i, place, me.y, me.j, hi, L);
+    for (int o = 0; o < cluster; ++o)
+      if (o != r) place += place_of(lists[o], parts[o].count, me);
+    if (place < a.top) write_top(a, i, place, me, hi, L);
   }
 }
 
@@ -674,69 +828,132 @@ template <typename T> struct ScoreGradArgs {
 // The gradient reads and writes every score once: bound by HBM.  With t = log p in the
 // exponent's unit, dx = p (A + B t) with A = -scale (g_l + g_H H), B = -scale g_H, and
 // scale g_l more at the label: per score a subtraction, two fused multiply-adds, one
-// exponential and a product.  One warp per (row, kGradVecs 16-byte vectors a lane) of the
-// output, whose alignment decides where the vectors begin; scores whose row starts elsewhere
-// in its 16 bytes are read element by element.
+// exponential and a product, fp32 in pairs.  One warp per (row, kGradVecs 16-byte vectors a
+// lane) of the output, whose alignment decides where the vectors begin; scores whose row
+// starts elsewhere in its 16 bytes are read element by element.
 constexpr int kGradVecs = 4;
 
-template <typename T> __global__ void __launch_bounds__(256) scores_grad_kernel(ScoreGradArgs<T> a, int64_t chunks) {
+template <typename A> struct GradRow {
+  A h, c, nL, ca, cb;  // t = (x - h) c + nL, h and c with the scale's sign
+};
+
+// y <- p (A + B t)
+template <int N> __device__ __forceinline__ void grad_values(float* y, const GradRow<float>& r) {
+  const uint64_t h = f2_pack(r.h, r.h), c = f2_pack(r.c, r.c), nl = f2_pack(r.nL, r.nL), ca = f2_pack(r.ca, r.ca),
+                 cb = f2_pack(r.cb, r.cb);
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    float t0, t1;
+    f2_unpack(f2_fma(f2_sub(f2_pack(y[e], y[e + 1]), h), c, nl), t0, t1);
+    t0 = fmaxf(t0, Expo<float>::floor);
+    t1 = fmaxf(t1, Expo<float>::floor);
+    const uint64_t p = f2_pack(Expo<float>::exp(t0), Expo<float>::exp(t1));
+    f2_unpack(f2_mul(p, f2_fma(cb, f2_pack(t0, t1), ca)), y[e], y[e + 1]);
+  }
+}
+template <int N> __device__ __forceinline__ void grad_values(double* y, const GradRow<double>& r) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    double t = (y[e] - r.h) * r.c + r.nL;
+    t = t > Expo<double>::floor ? t : Expo<double>::floor;
+    y[e] = Expo<double>::exp(t) * (r.ca + r.cb * t);
+  }
+}
+
+template <typename T> __device__ __forceinline__ uint4 pack(const Acc<T>* y) {
+  Vec<T, 16 / static_cast<int>(sizeof(T))> v;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&v.raw);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[q] = __floats2bfloat162_rn(y[2 * q], y[2 * q + 1]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    __half2* p = reinterpret_cast<__half2*>(&v.raw);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[q] = __floats2half2_rn(y[2 * q], y[2 * q + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) v.e[e] = y[e];
+  }
+  return v.raw;
+}
+
+template <typename T> __global__ void __launch_bounds__(256) scores_grad_kernel(ScoreGradArgs<T> a, int chunks) {
   using A = Acc<T>;
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
   const int lane = threadIdx.x & 31;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int64_t i = unit / chunks;
   if (i >= a.n) return;
-  const int64_t chunk = unit - i * chunks;
+  const int chunk = static_cast<int>(unit - i * chunks);
   T* out = a.grad + i * a.m;
   const T* x = a.x + i * a.ld;
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
-  const bool same = (reinterpret_cast<uintptr_t>(x) & 15u) == (reinterpret_cast<uintptr_t>(out) & 15u);
-  const int64_t j0 = chunk * (32 * kGradVecs * VE) + lane * VE - off;
-  Vec<T, VE> v[kGradVecs];
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int j0 = (chunk * (32 * kGradVecs) + lane) * VE - off;
+  const bool whole = j0 >= 0 && j0 + (kGradVecs - 1) * 32 * VE + VE <= a.m;
+  uint4 w[kGradVecs];
+  if (whole && same) {
+    const uint4* from = reinterpret_cast<const uint4*>(x + j0);
 #pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int64_t j = j0 + u * 32 * VE;
-    if (same && j >= 0 && j + VE <= a.m) {
-      v[u].raw = load_once(reinterpret_cast<const uint4*>(x + j));
-    } else {
+    for (int u = 0; u < kGradVecs; ++u) w[u] = load_once(from + u * 32);
+  } else {
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (j + e >= 0 && j + e < a.m) v[u].e[e] = x[j + e];
+    for (int u = 0; u < kGradVecs; ++u) {
+      Vec<T, VE> v;
+      v.raw = raw_zero<uint4>();
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const int j = j0 + u * 32 * VE + e;
+        if (j >= 0 && j < a.m) v.e[e] = x[j];
+      }
+      w[u] = v.raw;
     }
   }
   const A hi = a.stats[3 * i], L = a.stats[3 * i + 1], H = a.stats[3 * i + 2];
-  const int64_t l = a.labels ? label_of<T>(a.labels, a.labels_i64, i) : -1;
-  const A gl = l >= 0 && l < a.m && a.g_log_probs ? a.g_log_probs[i] : A(0);
+  const int64_t label = a.labels ? label_of<T>(a.labels, a.labels_i64, i) : -1;
+  const bool has = label >= 0 && label < a.m && a.g_log_probs;
+  const A gl = has ? a.g_log_probs[i] : A(0);
   const A gh = a.g_entropy ? a.g_entropy[i] : A(0);
-  const A scale = a.sign * a.mag, c = a.mag * Expo<A>::per_nat, L2 = L * Expo<A>::per_nat;
-  const bool empty = hi == neg_inf<A>();
-  const A ca = -scale * (gl + gh * H), cb = -scale * gh * Expo<A>::unit;
+  const A scale = a.sign * a.mag;
+  GradRow<A> r;  // of an empty row (hi = -inf) every t is the floor, and p 0
+  r.h = a.sign * hi;
+  r.c = a.sign * (a.mag * Expo<A>::per_nat);
+  r.nL = -L * Expo<A>::per_nat;
+  r.ca = -scale * (gl + gh * H);
+  r.cb = -scale * gh * Expo<A>::unit;
+  const int hit = has && hi != neg_inf<A>() ? static_cast<int>(label) - j0 : -1;
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
-    const int64_t j = j0 + u * 32 * VE;
-    if (j >= a.m || j + VE <= 0) continue;
+    A y[VE];
+    unpack<T>(w[u], y);
+    grad_values<VE>(y, r);
+    if (static_cast<unsigned>(hit - u * 32 * VE) < static_cast<unsigned>(VE)) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      A t = (a.sign * to_acc(v[u].e[e]) - hi) * c - L2;
-      t = t > Expo<A>::floor ? t : Expo<A>::floor;
-      A dx = Expo<A>::exp(t) * (ca + cb * t);
-      if (j + e == l) dx += scale * gl;
-      v[u].e[e] = from_acc<T>(empty ? A(0) : dx);
+      for (int e = 0; e < VE; ++e)
+        if (e == hit - u * 32 * VE) y[e] += scale * gl;
     }
-    if (j >= 0 && j + VE <= a.m) {
-      store_once(reinterpret_cast<uint4*>(out + j), v[u].raw);
+    const int j = j0 + u * 32 * VE;
+    if (whole || (j >= 0 && j + VE <= a.m)) {
+      store_once(reinterpret_cast<uint4*>(out + j), pack<T>(y));
     } else {
 #pragma unroll
       for (int e = 0; e < VE; ++e)
-        if (j + e >= 0 && j + e < a.m) out[j + e] = v[u].e[e];
+        if (j + e >= 0 && j + e < a.m) out[j + e] = from_acc<T>(y[e]);
     }
   }
 }
 
 // ------------------------------------------------------------------ launches
-template <typename T, int EPL> static cudaError_t scores_warp(const ScoreArgs<T>& a, cudaStream_t st) {
-  const int64_t blocks = std::min<int64_t>((a.n + 3) / 4, static_cast<int64_t>(num_sms()) * 64);
-  scores_warp_kernel<T, EPL><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
+template <typename T, int TEAM, int EPL> static cudaError_t scores_team(const ScoreArgs<T>& a, cudaStream_t st) {
+  constexpr int VE = RowVecs<T>::VE;
+  const unsigned blocks =
+      static_cast<unsigned>(std::min<int64_t>((a.n * TEAM + 127) / 128, static_cast<int64_t>(num_sms()) * 20));
+  const bool flat =
+      a.m % VE == 0 && ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ld * sizeof(T))) & 15u) == 0;
+  if (flat)
+    scores_team_kernel<T, TEAM, EPL, true><<<blocks, 128, 0, st>>>(a);
+  else
+    scores_team_kernel<T, TEAM, EPL, false><<<blocks, 128, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -772,7 +989,9 @@ template <typename T, int NT> static cudaError_t scores_block(const ScoreArgs<T>
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, scores_block_kernel<T, NT>, a, cluster, per_group);
+  int log_cluster = 0;
+  while ((1 << log_cluster) < cluster) ++log_cluster;
+  return cudaLaunchKernelEx(&cfg, scores_block_kernel<T, NT>, a, log_cluster, per_group);
 }
 
 template <typename T> static cudaError_t scores_t(const ScoreJob& j, cudaStream_t st) {
@@ -791,15 +1010,17 @@ template <typename T> static cudaError_t scores_t(const ScoreJob& j, cudaStream_
   a.stats = static_cast<Acc<T>*>(j.stats);
   a.top_log_probs = static_cast<Acc<T>*>(j.top_log_probs);
   a.top_labels = j.top_labels;
-  // a row in one warp's registers where it fits at any alignment of its rows
-  const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ld * sizeof(T))) & 15u) == 0;
-  const int64_t span = a.m + (aligned ? 0 : RowVecs<T>::VE - 1);
-  if (span <= 32 * 8) return scores_warp<T, 8>(a, st);
-  if (span <= 32 * 16) return scores_warp<T, 16>(a, st);
-  if (span <= 32 * 32) return scores_warp<T, 32>(a, st);
+  // a row in one team's registers where it fits; 8 lanes bound few alternatives well
+  if (a.top <= 8 && a.m <= 64) return scores_team<T, 8, 8>(a, st);
+  if (a.top <= 8 && a.m <= 256) return scores_team<T, 8, 32>(a, st);
+  if (a.m <= 256) return scores_team<T, 32, 8>(a, st);
+  if (a.m <= 512) return scores_team<T, 32, 16>(a, st);
+  if (a.m <= 1024) return scores_team<T, 32, 32>(a, st);
   if constexpr (sizeof(T) < 8)
-    if (span <= 32 * 64) return scores_warp<T, 64>(a, st);
-  if (span <= 16384) return scores_block<T, 128>(a, st);
+    if (a.m <= 2048 && a.n >= num_sms() * 4) return scores_team<T, 32, 64>(a, st);
+  if (a.m <= 8192 && a.n >= num_sms() * 8) return scores_block<T, 64>(a, st);
+  if (a.n >= num_sms() * 4 && static_cast<int64_t>(a.m) * static_cast<int64_t>(sizeof(T)) <= 262144)
+    return scores_block<T, 128>(a, st);
   return scores_block<T, 256>(a, st);
 }
 
@@ -819,7 +1040,9 @@ template <typename T> static cudaError_t scores_grad_t(const ScoreGradJob& j, cu
   a.grad = static_cast<T*>(j.grad);
   // chunks of a row at any alignment of the output's rows
   constexpr int64_t per = 32 * kGradVecs * (16 / sizeof(T));
-  const int64_t chunks = (a.m + 16 / static_cast<int64_t>(sizeof(T)) - 1 + per - 1) / per;
+  constexpr int64_t VE = 16 / sizeof(T);
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.grad) & 15u) == 0 && a.m % VE == 0;
+  const int chunks = static_cast<int>((a.m + (aligned ? 0 : VE - 1) + per - 1) / per);
   scores_grad_kernel<T><<<static_cast<unsigned>((a.n * chunks + 7) / 8), 256, 0, st>>>(a, chunks);
   return cudaGetLastError();
 }

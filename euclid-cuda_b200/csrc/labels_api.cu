@@ -9,6 +9,7 @@
 namespace euc {
 
 constexpr int64_t kMaxIndex = 0x7ffffffell;  // sorted positions, slots and labels are int32
+constexpr int64_t kMaxScores = 1ll << 30;    // a row's elements and vectors are counted in int32
 constexpr int kMaxTop = 32;
 
 static int done(cudaError_t e, const char* where) {
@@ -40,7 +41,7 @@ static bool misaligned(int t, std::initializer_list<const void*> ps) {
 }
 
 static int scores_shape(int row_type, int64_t ld, int64_t n, int64_t m, double scale) {
-  if (n < 0 || n > kMaxIndex || m < 1 || m > kMaxIndex) return set_error(EUC_ERR_SHAPE, "scores: bad size");
+  if (n < 0 || n > kMaxIndex || m < 1 || m > kMaxScores) return set_error(EUC_ERR_SHAPE, "scores: bad size");
   if (ld < m && n > 1) return set_error(EUC_ERR_SHAPE, "scores: row stride below the row's length");
   if (!std::isfinite(scale) || scale == 0.0) return set_error(EUC_ERR_ARG, "scale must be finite and not 0");
   // the fp32 arithmetic holds |scale| and its multiple of log2(e) as normal numbers

@@ -341,7 +341,7 @@ EUC_API int euc_kmeanspp(const void* X, int x_is_f64, int64_t n, int64_t dim, in
  * Sums, weights and statistics are fp32, and fp64 for fp64 rows. */
 typedef enum { EUC_ROW_F32 = 0, EUC_ROW_F64 = 1, EUC_ROW_F16 = 2, EUC_ROW_BF16 = 3 } euc_row_type;
 
-/* Log probabilities of n rows of m scores (row stride ld >= m elements), z = scale * x:
+/* Log probabilities of n rows of m <= 2^30 scores (row stride ld >= m elements), z = scale * x:
  * a row of D of any distance operator takes scale = -1 / temperature.
  *   log_probs[i]     = z[i, l_i] - log sum_j exp z[i, j]   (0 where l_i is outside [0, m))
  *   entropy[i]       = - sum_j p_j log p_j
