@@ -20,41 +20,57 @@
 
 namespace euc {
 
-template <typename T, int N, typename TL>
+// R U vectors a lane in flight: their rows' labels, then the table's vectors, before any is
+// stored
+template <typename T, int N, typename TL, int R, int U, bool WIDE>
 __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ C, int64_t k, const TL* __restrict__ labels,
-                                                     int64_t n, int64_t nv, Acc<T> scale, T* __restrict__ out) {
+                                                     int64_t n, int64_t nv, int64_t chunks, Acc<T> scale,
+                                                     T* __restrict__ out) {
   using V = Vec<T, N>;
   using Raw = typename V::Raw;
   const Raw* Cr = reinterpret_cast<const Raw*>(C);
   Raw* Or = reinterpret_cast<Raw*>(out);
-  RowWalk w(static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<int64_t>(gridDim.x) * blockDim.x,
-            nv);
-  while (w.row < n) {
-    // four vectors in flight: their labels, then the table's vectors, before any is stored
-    int64_t at[4], src[4];
+  V x[R][U];
+  auto scaled = [&](V v) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      at[u] = -1;
-      src[u] = -1;
-      if (w.row < n) {
-        at[u] = w.row * nv + w.v;
-        const int64_t c = static_cast<int64_t>(labels[w.row]);
-        if (c >= 0 && c < k) src[u] = c * nv + w.v;
-        w.next();
+    for (int e = 0; e < N; ++e) v.e[e] = from_acc<T>(scale * to_acc(v.e[e]));
+    return v.raw;
+  };
+  if constexpr (WIDE) {
+    const WideRows<R, U> w(chunks);
+    int64_t c[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) c[r] = w.row + r < n ? static_cast<int64_t>(labels[w.row + r]) : -1;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[r][u].raw = raw_zero<Raw>();
+        if (c[r] >= 0 && c[r] < k && w.v + 32 * u < nv) x[r][u].raw = load_keep(Cr + c[r] * nv + w.v + 32 * u);
       }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (w.row + r < n && w.v + 32 * u < nv)
+          store_once(Or + (w.row + r) * nv + w.v + 32 * u, c[r] >= 0 && c[r] < k ? scaled(x[r][u]) : raw_zero<Raw>());
+  } else {
+    const NarrowRows<U> w(nv);
+    int64_t row[U], c[U];
+    uint32_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w.at(u, row[u], v[u]);
+      c[u] = row[u] < n ? static_cast<int64_t>(labels[row[u]]) : -1;
     }
-    V v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u].raw = src[u] >= 0 ? load_keep(Cr + src[u]) : raw_zero<Raw>();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (at[u] < 0) continue;
-      if (src[u] >= 0) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[u].e[e] = from_acc<T>(scale * to_acc(v[u].e[e]));
-      }
-      store_once(Or + at[u], v[u].raw);
+    for (int u = 0; u < U; ++u) {
+      x[0][u].raw = raw_zero<Raw>();
+      if (c[u] >= 0 && c[u] < k) x[0][u].raw = load_keep(Cr + c[u] * nv + v[u]);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (row[u] < n) store_once(Or + row[u] * nv + v[u], c[u] >= 0 && c[u] < k ? scaled(x[0][u]) : raw_zero<Raw>());
   }
 }
 
@@ -68,37 +84,70 @@ struct GradArgs {
   int64_t chunks;
 };
 
+// zero rows for the labels without rows, a warp per label and 32 vectors at a time
+template <typename Raw>
+__device__ __forceinline__ void clear_rows(const GradArgs& a, int64_t block, int64_t blocks, Raw* out) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // 32 labels per warp: their emptiness is one ballot
+  for (int64_t c0 = (block * 8 + warp) * 32; c0 < a.k; c0 += blocks * 256) {
+    const int64_t c = c0 + lane;
+    const bool empty = c < a.k && a.offsets[c + 1] <= a.offsets[c];
+    unsigned todo = __ballot_sync(0xffffffffu, empty);
+    if (a.nv < 32) {  // short rows: neighbouring lanes over the vectors of all 32 labels
+      const uint32_t nv = static_cast<uint32_t>(a.nv);
+      for (uint32_t f = lane; f < 32 * nv && todo; f += 32)
+        if (todo >> (f / nv) & 1u) store_once(out + c0 * a.nv + f, raw_zero<Raw>());
+      continue;
+    }
+    while (todo) {
+      Raw* row = out + (c0 + __ffs(todo) - 1) * a.nv;
+      for (int64_t v = lane; v < a.nv; v += 32) store_once(row + v, raw_zero<Raw>());
+      todo &= todo - 1;
+    }
+  }
+}
+
 template <typename T, int N>
-__global__ void __launch_bounds__(256) grad_chunks_kernel(const T* __restrict__ G, GradArgs a, Acc<T> scale,
-                                                          T* __restrict__ out, Acc<T>* __restrict__ part) {
+__global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3 : 4)
+    grad_chunks_kernel(const T* __restrict__ G, GradArgs a, int64_t chunk_blocks, Acc<T> scale, T* __restrict__ out,
+                       Acc<T>* __restrict__ part) {
   using A = Acc<T>;
   using V = Vec<T, N>;
   using Raw = typename V::Raw;
   const Raw* Gr = reinterpret_cast<const Raw*>(G);
+  Raw* Or = reinterpret_cast<Raw*>(out);
+  if (static_cast<int64_t>(blockIdx.x) >= chunk_blocks) {
+    clear_rows<Raw>(a, blockIdx.x - chunk_blocks, gridDim.x - chunk_blocks, Or);
+    return;
+  }
   const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
   const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t chunk = t / a.nv, v = t - chunk * a.nv;
+  const int64_t chunk = t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(a.nv) : t / a.nv;
+  const int64_t v = t - chunk * a.nv;
   const int64_t p0 = chunk * a.seg;
   if (p0 >= total) return;
   const int64_t p1 = min(total, p0 + a.seg);
   A acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = A(0);
-  int64_t c = a.labels[p0];
+  int c = a.labels[p0];
+  // only the chunk's first label can have begun before it, only its last can go on behind it
+  bool from_left = p0 > 0 && a.labels[p0 - 1] == c;
+  const int behind = p1 < total ? a.labels[p1] : -1;
   auto flush = [&]() {
     if (c >= 0 && c < a.k) {
-      const int64_t lo = a.offsets[c], hi = a.offsets[c + 1];
-      if (lo >= p0 && hi <= p1) {
+      if (!from_left && c != behind) {
         V o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
-        store_once(reinterpret_cast<Raw*>(out) + c * a.nv + v, o.raw);
+        store_once(Or + c * a.nv + v, o.raw);
       } else {
-        A* to = part + ((2 * chunk + (lo < p0 ? 0 : 1)) * a.nv + v) * N;
+        A* to = part + ((2 * chunk + (from_left ? 0 : 1)) * a.nv + v) * N;
 #pragma unroll
         for (int e = 0; e < N; ++e) to[e] = acc[e];
       }
     }
+    from_left = false;
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = A(0);
   };
@@ -127,54 +176,118 @@ __global__ void __launch_bounds__(256) grad_chunks_kernel(const T* __restrict__ 
   flush();
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, Acc<T> scale, const Acc<T>* __restrict__ part,
-                                                        T* __restrict__ out) {
-  using A = Acc<T>;
-  using V = Vec<T, N>;
-  using Raw = typename V::Raw;
-  RowWalk w(static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<int64_t>(gridDim.x) * blockDim.x,
-            a.nv);
-  for (; w.row < a.k; w.next()) {
-    const int64_t lo = max(0, a.offsets[w.row]), hi = min(a.n, static_cast<int64_t>(a.offsets[w.row + 1]));
-    Raw* to = reinterpret_cast<Raw*>(out) + w.row * a.nv + w.v;
-    if (hi <= lo) {
-      store_once(to, raw_zero<Raw>());
-      continue;
+// A label that crosses chunks' borders is joined at the first border inside it: by the
+// thread of (border, vector) if it has at most kLongChunks chunks more, else by the block
+// that belongs to the first multiple of kLongChunks among its chunks, whose lanes take
+// neighbouring vectors, its other threads every so-manyth chunk, and whose sums are added in
+// a fixed order.
+constexpr int kLongChunks = 16;
+
+// sum over chunks [c, c1], every `step`-th, of the label that starts at position lo
+template <typename A, int N>
+__device__ __forceinline__ void add_parts(const A* part, int64_t c, int64_t c1, int64_t step, int64_t lo, int seg,
+                                          int64_t nv, int64_t v, A* acc) {
+  for (; c <= c1; c += 4 * step) {
+    A from[4][N];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t q = c + u * step;
+      const A* at = part + ((2 * q + (lo < q * seg ? 0 : 1)) * nv + v) * N;
+#pragma unroll
+      for (int e = 0; e < N; ++e) from[u][e] = q <= c1 ? at[e] : A(0);
     }
-    const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
-    if (c0 == c1) continue;  // written by its chunk
-    A acc[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = A(0);
-    for (int64_t c = c0; c <= c1; ++c) {
-      const A* from = part + ((2 * c + (lo < c * a.seg ? 0 : 1)) * a.nv + w.v) * N;
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += from[e];
-    }
-    V o;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
-    store_once(to, o.raw);
+      for (int e = 0; e < N; ++e) acc[e] += from[u][e];
   }
 }
 
-// ------------------------------------------------------------------ launches
-static unsigned grid_for(int64_t items, int waves) {
-  const int64_t most = static_cast<int64_t>(num_sms()) * waves;
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, most)));
+template <typename T, int N>
+__device__ __forceinline__ void join_long(const GradArgs& a, int64_t block, Acc<T> scale,
+                                          const Acc<T>* __restrict__ part, T* __restrict__ out) {
+  using A = Acc<T>;
+  using V = Vec<T, N>;
+  __shared__ A sums[256][N];
+  // lanes over vectors: the power of two that holds the row, at most a warp
+  int width = 32;
+  while (width > 1 && width / 2 >= a.nv) width /= 2;
+  const int64_t tiles = (a.nv + width - 1) / width;
+  const int64_t chunk = block / tiles * kLongChunks;
+  const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
+  if (chunk * a.seg >= total) return;
+  const int64_t c = a.labels[chunk * a.seg];
+  if (c < 0 || c >= a.k) return;
+  const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
+  if (hi <= lo) return;
+  const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
+  // (chunk's first row has the label, so the multiple before it is the only other candidate)
+  if (c1 - c0 < kLongChunks || (chunk - kLongChunks) * a.seg >= lo) return;
+  const int groups = 256 / width, group = static_cast<int>(threadIdx.x) / width, lane = static_cast<int>(threadIdx.x) % width;
+  const int64_t v = block % tiles * width + lane;
+  A acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = A(0);
+  if (v < a.nv) add_parts<A, N>(part, c0 + group, c1, groups, lo, a.seg, a.nv, v, acc);
+#pragma unroll
+  for (int e = 0; e < N; ++e) sums[threadIdx.x][e] = acc[e];
+  for (int half = groups / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (group < half)
+#pragma unroll
+      for (int e = 0; e < N; ++e) sums[threadIdx.x][e] += sums[threadIdx.x + half * width][e];
+  }
+  if (group == 0 && v < a.nv) {
+    V o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * sums[threadIdx.x][e]);
+    store_once(reinterpret_cast<typename V::Raw*>(out) + c * a.nv + v, o.raw);
+  }
 }
 
-// Rows per chunk.
-static int grad_seg(int64_t n) {
+template <typename T, int N>
+__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int64_t long_blocks, Acc<T> scale,
+                                                        const Acc<T>* __restrict__ part, T* __restrict__ out) {
+  using A = Acc<T>;
+  using V = Vec<T, N>;
+  using Raw = typename V::Raw;
+  if (static_cast<int64_t>(blockIdx.x) < long_blocks) {  // the longest work starts first
+    join_long<T, N>(a, blockIdx.x, scale, part, out);
+    return;
+  }
+  const int64_t t = static_cast<int64_t>(blockIdx.x - long_blocks) * blockDim.x + threadIdx.x;
+  const int64_t border = 1 + (t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(a.nv) : t / a.nv);
+  const int64_t v = t - (border - 1) * a.nv, at = border * a.seg;
+  if (at >= min(a.n, static_cast<int64_t>(a.offsets[a.k]))) return;
+  const int64_t c = a.labels[at];
+  if (c < 0 || c >= a.k || a.labels[at - 1] != c) return;
+  const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
+  const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
+  if (c0 != border - 1 || c1 - c0 >= kLongChunks) return;  // an earlier border's, or a block's
+  A acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = A(0);
+  add_parts<A, N>(part, c0, c1, 1, lo, a.seg, a.nv, v, acc);
+  V o;
+#pragma unroll
+  for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
+  store_once(reinterpret_cast<Raw*>(out) + c * a.nv + v, o.raw);
+}
+
+// ------------------------------------------------------------------ launches
+// Rows per chunk: as many as leave 32 warps per SM, since every chunk may cost two partial
+// sums and their join.  `row_bytes` / 16 stands for the row's vectors at any alignment.
+static int grad_seg(int64_t n, int64_t row_bytes) {
+  const int64_t nv = std::max<int64_t>(1, row_bytes / 16);
   int seg = 16;
-  while (seg < 256 && n / seg > 8192) seg *= 2;
+  while (seg < 256 && n / (2 * seg) * nv >= static_cast<int64_t>(num_sms()) * 1024) seg *= 2;
   return seg;
 }
 
 size_t codebook_grad_ws_bytes(RowType t, int64_t n, int64_t dim) {
   if (n <= 0) return 0;
-  const int64_t chunks = (n + grad_seg(n) - 1) / grad_seg(n);
+  const int64_t seg = grad_seg(n, dim * (t == ROW_F64 ? 8 : t == ROW_F32 ? 4 : 2));
+  const int64_t chunks = (n + seg - 1) / seg;
   return static_cast<size_t>(2 * chunks) * dim * (t == ROW_F64 ? 8 : 4);
 }
 
@@ -182,9 +295,22 @@ template <typename T, int N, typename TL>
 static cudaError_t lookup_go(const T* C, int64_t k, const TL* labels, int64_t n, int64_t dim, double scale, T* out,
                              cudaStream_t st) {
   const int64_t nv = dim / N;
-  lookup_kernel<T, N, TL><<<grid_for((n * nv + 3) / 4, 64), 256, 0, st>>>(C, k, labels, n, nv,
-                                                                        static_cast<Acc<T>>(scale), out);
-  return cudaGetLastError();
+  const Acc<T> s = static_cast<Acc<T>>(scale);
+  auto wide = [&](auto kernel, int R, int U) {
+    kernel<<<static_cast<unsigned>(wide_blocks(n, nv, R, U)), 256, 0, st>>>(C, k, labels, n, nv,
+                                                                          (nv + 32 * U - 1) / (32 * U), s, out);
+    return cudaGetLastError();
+  };
+  if (nv < 32) {
+    lookup_kernel<T, N, TL, 1, 4, false>
+        <<<static_cast<unsigned>(narrow_blocks(n, nv, 4)), 256, 0, st>>>(C, k, labels, n, nv, 1, s, out);
+    return cudaGetLastError();
+  }
+  // few rows are spread over more warps: latency counts there, not what a warp has in flight
+  if (n * nv <= static_cast<int64_t>(num_sms()) * 2048) return wide(lookup_kernel<T, N, TL, 1, 1, true>, 1, 1);
+  if (nv <= 32) return wide(lookup_kernel<T, N, TL, 4, 1, true>, 4, 1);
+  if (nv <= 64) return wide(lookup_kernel<T, N, TL, 2, 2, true>, 2, 2);
+  return wide(lookup_kernel<T, N, TL, 1, 4, true>, 1, 4);
 }
 
 template <typename T, int N>
@@ -199,11 +325,17 @@ static cudaError_t grad_n(const T* G, GradArgs a, int64_t dim, double scale, T* 
   a.nv = dim / N;
   Acc<T>* part = static_cast<Acc<T>*>(ws);
   const Acc<T> s = static_cast<Acc<T>>(scale);
-  if (a.n > 0) {
-    const int64_t threads = a.chunks * a.nv;
-    grad_chunks_kernel<T, N><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, st>>>(G, a, s, out, part);
+  const int64_t sums = (a.chunks * a.nv + 255) / 256;
+  const int64_t clears = std::min<int64_t>((a.k + 255) / 256, static_cast<int64_t>(num_sms()) * 8);
+  grad_chunks_kernel<T, N><<<static_cast<unsigned>(sums + clears), 256, 0, st>>>(G, a, sums, s, out, part);
+  if (a.chunks > 1) {
+    int width = 32;
+    while (width > 1 && width / 2 >= a.nv) width /= 2;
+    const int64_t longs =
+        a.chunks > kLongChunks ? (a.chunks + kLongChunks - 1) / kLongChunks * ((a.nv + width - 1) / width) : 0;
+    const int64_t shorts = ((a.chunks - 1) * a.nv + 255) / 256;
+    grad_join_kernel<T, N><<<static_cast<unsigned>(longs + shorts), 256, 0, st>>>(a, longs, s, part, out);
   }
-  grad_join_kernel<T, N><<<grid_for(a.k * a.nv, 64), 256, 0, st>>>(a, s, part, out);
   return cudaGetLastError();
 }
 
@@ -242,7 +374,7 @@ cudaError_t launch_codebook_grad(RowType t, const void* G, const int32_t* offset
   a.labels = sorted;
   a.n = n;
   a.k = k;
-  a.seg = grad_seg(n);
+  a.seg = grad_seg(n, dim * (t == ROW_F64 ? 8 : t == ROW_F32 ? 4 : 2));
   a.chunks = (n + a.seg - 1) / a.seg;
   switch (t) {
     case ROW_F32: return grad_t<float>(G, a, dim, scale, out, ws, st);

@@ -11,12 +11,16 @@
 // and dX[i] = sum_j dY[position[i, j]], the second with weights of one.
 //
 // The sort is a counting sort in passes of up to kMaxBins bins (one pass for k < kMaxBins,
-// else 2 or 3 by digits, least significant first): per tile of slots a histogram, a scan
-// of each bin over the tiles, and a scatter that ranks a slot among its tile's equal keys
-// by __match_any_sync within 32 slots, in slot order.  It moves 4 to 8 bytes a slot where
-// the rows move kilobytes; the row kernels are bound by HBM, and read and write every row
-// once: a row's copies are written from registers after one read, and its weighted sum is
-// formed from p reads and written once.
+// else 2 or 3 by digits, least significant first); a slot is ranked among its warp's equal
+// keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit counters per warp
+// and bin.  Up to kClusterSlots slots one cluster of at most 8 blocks runs all passes: the
+// blocks' totals are exchanged through distributed shared memory, so a pass costs two
+// cluster barriers and no launch.  More slots take three kernels a pass (histograms of
+// tiles, scan of each bin over the tiles, scatter through shared memory so that a bin's run
+// is stored together).  The sort moves 4 to 8 bytes a slot where the rows move kilobytes;
+// the row kernels are bound by HBM, and read and write every row once: a row's copies are
+// written from registers after one read, its weighted sum is formed from p reads.
+#include "common.cuh"
 #include "engine.h"
 #include "rows.cuh"
 
@@ -25,62 +29,20 @@
 namespace euc {
 
 // ------------------------------------------------------------------ the sort
-constexpr int kMaxBins = 4097;   // k + 1 bins (the last for labels outside [0, k)) in one pass
-constexpr int kSortWarps = 8;
-constexpr int kSortItems = 16;   // slots per thread
-constexpr int kTile = kSortWarps * 32 * kSortItems;
+constexpr int kMaxBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass
+constexpr int kPassBits = 11;   // digits of a sort of several passes, at most
 
-struct SortPass {
-  int64_t n;
-  uint32_t k;       // keys lie in [0, k]; k marks a dropped slot
-  int shift;
-  uint32_t mask;
-  int bins;
-  int tiles;
-  uint32_t* T;      // [bins][tiles] counts, then exclusive prefixes over the tiles
-  uint32_t* total;  // [bins]
+struct SortOut {
+  uint32_t* keys;  // a pass that is not the last: keys and slots in the pass's order
+  uint32_t* slots;
+  int32_t* order;  // the last pass
+  int32_t* position;
+  int32_t* labels;
+  int32_t* offsets;  // a sort of one pass, else null
 };
 
 template <typename TL> __device__ __forceinline__ uint32_t key_of(TL label, uint32_t k) {
   return label >= 0 && label < static_cast<TL>(k) ? static_cast<uint32_t>(label) : k;
-}
-// the keys of a later pass
-template <> __device__ __forceinline__ uint32_t key_of<uint32_t>(uint32_t key, uint32_t) { return key; }
-
-template <typename TL>
-__global__ void __launch_bounds__(kSortWarps * 32) sort_hist_kernel(const TL* __restrict__ in, SortPass a) {
-  extern __shared__ uint32_t cnt[];
-  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) cnt[c] = 0u;
-  __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-#pragma unroll
-  for (int u = 0; u < kSortItems; ++u) {
-    const int64_t s = base + u * (kSortWarps * 32) + threadIdx.x;
-    if (s < a.n) atomicAdd(&cnt[(key_of(in[s], a.k) >> a.shift) & a.mask], 1u);
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] = cnt[c];
-}
-
-// one warp per bin: T[bin][.] becomes its exclusive prefix over the tiles
-__global__ void __launch_bounds__(256) sort_tiles_kernel(SortPass a) {
-  const int bin = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (bin >= a.bins) return;
-  uint32_t* row = a.T + static_cast<int64_t>(bin) * a.tiles;
-  uint32_t run = 0u;
-  for (int b0 = 0; b0 < a.tiles; b0 += 32) {
-    const int b = b0 + lane;
-    const uint32_t v = b < a.tiles ? row[b] : 0u;
-    uint32_t x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (b < a.tiles) row[b] = run + x - v;
-    run += __shfl_sync(0xffffffffu, x, 31);
-  }
-  if (lane == 0) a.total[bin] = run;
 }
 
 // exclusive scan of v[0, m) in shared memory by the whole block (m of any size)
@@ -98,9 +60,8 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int m, uint32_t* warp_su
   }
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  uint32_t before = 0u;
-  for (int w = 0; w < nw; ++w) before += w < warp ? warp_sums[w] : 0u;
-  uint32_t run = before + x - sum;
+  uint32_t run = x - sum;
+  for (int w = 0; w < nw; ++w) run += w < warp ? warp_sums[w] : 0u;
   for (int c = lo; c < hi; ++c) {
     const uint32_t t = v[c];
     v[c] = run;
@@ -109,78 +70,262 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int m, uint32_t* warp_su
   __syncthreads();
 }
 
-struct SortOut {
-  uint32_t* keys;      // a pass that is not the last: keys and slots in the pass's order
-  uint32_t* slots;
-  int32_t* order;      // the last pass
-  int32_t* position;
-  int32_t* labels;
-  int32_t* offsets;    // the last pass of a one-pass sort, else null
+// rank[u] <- slots of the warp before (u, lane) with its digit; counts <- slots per digit
+template <int ITEMS>
+__device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], unsigned short (&rank)[ITEMS],
+                                           unsigned short* counts, int lane) {
+#pragma unroll
+  for (int u = 0; u < ITEMS; ++u) {
+    const bool in = digit[u] != 0xffffffffu;
+    const unsigned peers = __match_any_sync(0xffffffffu, digit[u]);
+    const int before = __popc(peers & ((1u << lane) - 1u));
+    unsigned short base = 0;
+    if (in) base = counts[digit[u]];
+    __syncwarp();
+    if (in && before == 0) counts[digit[u]] = static_cast<unsigned short>(base + __popc(peers));
+    rank[u] = static_cast<unsigned short>(base + before);
+    __syncwarp();
+  }
+}
+
+// ---- all passes in one cluster
+struct ClusterSort {
+  int64_t n;
+  uint32_t k;
+  int passes, bits, bins, log_cluster;
+  uint32_t *keys[2], *slots[2];  // between passes
 };
 
+constexpr int kClusterItems = 2;
+constexpr int64_t kClusterSlots = 8 * 1024 * kClusterItems;  // more scatter faster from every SM than from eight
+
+template <typename TL, int ITEMS>
+__global__ void __launch_bounds__(1024) sort_cluster_kernel(const TL* __restrict__ in, ClusterSort a, SortOut o) {
+  extern __shared__ uint32_t sm[];
+  __shared__ uint32_t warp_sums[32];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cluster = 1 << a.log_cluster, rank_in = static_cast<int>(blockIdx.x);
+  uint32_t* total = sm;               // [bins] this block's slots per digit
+  uint32_t* start = sm + a.bins;      // [bins] first position of this block's slots
+  uint32_t* before = sm + 2 * a.bins;  // [bins] slots of the cluster's earlier blocks per digit
+  unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + 3 * a.bins);  // [warps][bins]
+  unsigned short* mine = cnt + warp * a.bins;
+  const int64_t base = (static_cast<int64_t>(rank_in) * warps + warp) * (32 * ITEMS) + lane;
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const bool last = pass == a.passes - 1;
+    const int shift = pass * a.bits;
+    const uint32_t mask = a.passes == 1 ? 0xffffffffu : (1u << a.bits) - 1u;
+    const uint32_t* from_keys = a.keys[(pass + 1) & 1];
+    const uint32_t* from_slots = a.slots[(pass + 1) & 1];
+    uint32_t key[ITEMS], digit[ITEMS];
+    unsigned short rank[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int64_t s = base + u * 32;
+      key[u] = s >= a.n ? 0u : pass == 0 ? key_of(in[s], a.k) : __ldcg(from_keys + s);
+      digit[u] = s >= a.n ? 0xffffffffu : (key[u] >> shift) & mask;
+    }
+    for (int c = threadIdx.x; c < a.bins * warps; c += blockDim.x) cnt[c] = 0;
+    __syncthreads();
+    warp_ranks<ITEMS>(digit, rank, mine, lane);
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
+      uint32_t run = 0;
+      for (int w = 0; w < warps; ++w) {
+        const unsigned short t = cnt[w * a.bins + c];
+        cnt[w * a.bins + c] = static_cast<unsigned short>(run);
+        run += t;
+      }
+      total[c] = run;
+      start[c] = run;
+    }
+    __syncthreads();
+    if (cluster > 1) {
+      cluster_sync();
+      for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {
+        uint32_t all = 0u, earlier = 0u;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t t = r < cluster ? load_cluster_u32(total + c, static_cast<uint32_t>(r)) : 0u;
+          all += t;
+          earlier += r < rank_in ? t : 0u;
+        }
+        start[c] = all;
+        before[c] = earlier;
+      }
+      __syncthreads();
+    }
+    block_scan(start, a.bins, warp_sums);
+    if (last && o.offsets && rank_in == 0)
+      for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int64_t s = base + u * 32;
+      if (s >= a.n) continue;
+      const uint32_t pos = start[digit[u]] + (cluster > 1 ? before[digit[u]] : 0u) + mine[digit[u]] + rank[u];
+      const uint32_t slot = pass == 0 ? static_cast<uint32_t>(s) : __ldcg(from_slots + s);
+      if (last) {
+        const bool kept = key[u] < a.k;
+        o.order[pos] = kept ? static_cast<int32_t>(slot) : -1;
+        o.labels[pos] = kept ? static_cast<int32_t>(key[u]) : -1;
+        o.position[slot] = kept ? static_cast<int32_t>(pos) : -1;
+      } else {
+        a.keys[pass & 1][pos] = key[u];
+        a.slots[pass & 1][pos] = slot;
+      }
+    }
+    // the next pass reads what every block wrote, and none leaves while its totals are read
+    __syncthreads();
+    if (cluster > 1) cluster_sync();
+  }
+}
+
+// ---- three kernels a pass
+constexpr int kTileWarps = 8;
+constexpr int kTileItems = 8;
+constexpr int kTile = kTileWarps * 32 * kTileItems;  // 2048 slots, so 16 bits index one of them
+
+struct SortPass {
+  int64_t n;
+  uint32_t k;  // keys lie in [0, k]; k marks a dropped slot
+  int shift;
+  uint32_t mask;
+  int bins;
+  int tiles;        // rounded up to whole 16 bytes of T
+  uint32_t* T;      // [bins][tiles] counts, then exclusive prefixes over the tiles
+  uint32_t* total;  // [bins]
+};
+
+template <typename TL, bool FIRST> __device__ __forceinline__ uint32_t load_key(const TL* in, int64_t s, uint32_t k) {
+  if constexpr (FIRST) return key_of(in[s], k);
+  else return static_cast<uint32_t>(in[s]);
+}
+
+template <typename TL, bool FIRST>
+__global__ void __launch_bounds__(kTileWarps * 32) sort_hist_kernel(const TL* __restrict__ in, SortPass a) {
+  extern __shared__ uint32_t cnt[];
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) cnt[c] = 0u;
+  __syncthreads();
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x;
+  uint32_t key[kTileItems];
+#pragma unroll
+  for (int u = 0; u < kTileItems; ++u) {
+    const int64_t s = base + u * (kTileWarps * 32);
+    key[u] = s < a.n ? load_key<TL, FIRST>(in, s, a.k) : 0u;
+  }
+#pragma unroll
+  for (int u = 0; u < kTileItems; ++u)
+    if (base + u * (kTileWarps * 32) < a.n) atomicAdd(&cnt[(key[u] >> a.shift) & a.mask], 1u);
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {
+    uint32_t* row = a.T + static_cast<int64_t>(c) * a.tiles;
+    row[blockIdx.x] = cnt[c];
+    if (blockIdx.x == gridDim.x - 1)  // the padding
+      for (int t = gridDim.x; t < a.tiles; ++t) row[t] = 0u;
+  }
+}
+
+// one warp per bin: T[bin][.] becomes its exclusive prefix over the tiles, 512 tiles at a time
+__global__ void __launch_bounds__(256) sort_tiles_kernel(SortPass a) {
+  const int bin = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (bin >= a.bins) return;
+  uint4* row = reinterpret_cast<uint4*>(a.T + static_cast<int64_t>(bin) * a.tiles);
+  const int quads = a.tiles / 4;
+  uint32_t run = 0u;
+  for (int b0 = 0; b0 < quads; b0 += 128) {
+    uint4 v[4];
+    uint32_t x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int b = b0 + u * 32 + lane;
+      v[u] = b < quads ? row[b] : make_uint4(0u, 0u, 0u, 0u);
+      x[u] = v[u].x + v[u].y + v[u].z + v[u].w;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x[u], o);
+        if (lane >= o) x[u] += y;
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int b = b0 + u * 32 + lane;
+      uint4 w;
+      w.x = run + x[u] - (v[u].x + v[u].y + v[u].z + v[u].w);
+      w.y = w.x + v[u].x;
+      w.z = w.y + v[u].y;
+      w.w = w.z + v[u].z;
+      if (b < quads) row[b] = w;
+      run += __shfl_sync(0xffffffffu, x[u], 31);
+    }
+  }
+  if (lane == 0) a.total[bin] = run;
+}
+
 template <typename TL, bool FIRST, bool LAST>
-__global__ void __launch_bounds__(kSortWarps * 32) sort_scatter_kernel(const TL* __restrict__ in,
+__global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL* __restrict__ in,
                                                                       const uint32_t* __restrict__ in_slots,
                                                                       SortPass a, SortOut o) {
   extern __shared__ uint32_t sm[];
-  __shared__ uint32_t warp_sums[kSortWarps];
-  uint32_t* start = sm;                                             // [bins] first position of the tile's bin
-  unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + a.bins);  // [warps][bins]
+  __shared__ uint32_t warp_sums[kTileWarps];
+  uint32_t* start = sm;                  // [bins] global position of the tile's first slot of the bin,
+  uint32_t* local = sm + a.bins;         // [bins] less its position in the tile
+  uint32_t* stage = sm + 2 * a.bins;     // [kTile] digit and slot, in the tile's order
+  unsigned short* cnt = reinterpret_cast<unsigned short*>(stage + kTile);  // [warps][bins]
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) start[c] = a.total[c];
-  for (int c = threadIdx.x; c < a.bins * kSortWarps; c += blockDim.x) cnt[c] = 0;
+  for (int c = threadIdx.x; c < a.bins * kTileWarps; c += blockDim.x) cnt[c] = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned short* mine = cnt + warp * a.bins;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) * kTile;
+  const int first = warp * (32 * kTileItems) + lane;
+  uint32_t digit[kTileItems];
+  unsigned short rank[kTileItems];
+#pragma unroll
+  for (int u = 0; u < kTileItems; ++u) {
+    const int64_t s = tile + first + u * 32;
+    digit[u] = s < a.n ? (load_key<TL, FIRST>(in, s, a.k) >> a.shift) & a.mask : 0xffffffffu;
+  }
   __syncthreads();
   block_scan(start, a.bins, warp_sums);
   if (LAST && o.offsets && blockIdx.x == 0)
     for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
-
-  // a warp's slots are contiguous, 32 at a time in slot order
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned short* mine = cnt + warp * a.bins;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + warp * (32 * kSortItems);
-  uint32_t key[kSortItems];
-  unsigned short rank[kSortItems];
-#pragma unroll
-  for (int u = 0; u < kSortItems; ++u) {
-    const int64_t s = base + u * 32 + lane;
-    key[u] = s < a.n ? key_of(in[s], a.k) : 0xffffffffu;
-  }
-#pragma unroll
-  for (int u = 0; u < kSortItems; ++u) {
-    const bool in_range = base + u * 32 + lane < a.n;
-    const uint32_t d = in_range ? (key[u] >> a.shift) & a.mask : 0xffffffffu;
-    const unsigned peers = __match_any_sync(0xffffffffu, d);
-    const int before = __popc(peers & ((1u << lane) - 1u));
-    if (in_range) rank[u] = static_cast<unsigned short>(mine[d] + before);
-    __syncwarp();
-    if (in_range && before == 0) mine[d] = static_cast<unsigned short>(mine[d] + __popc(peers));
-    __syncwarp();
-  }
+  warp_ranks<kTileItems>(digit, rank, mine, lane);
   __syncthreads();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
-    start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x];
-    unsigned short run = 0;
+    uint32_t run = 0;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
+    for (int w = 0; w < kTileWarps; ++w) {
       const unsigned short t = cnt[w * a.bins + c];
-      cnt[w * a.bins + c] = run;
-      run = static_cast<unsigned short>(run + t);
+      cnt[w * a.bins + c] = static_cast<unsigned short>(run);
+      run += t;
     }
+    local[c] = run;
   }
   __syncthreads();
+  block_scan(local, a.bins, warp_sums);
 #pragma unroll
-  for (int u = 0; u < kSortItems; ++u) {
-    const int64_t s = base + u * 32 + lane;
-    if (s >= a.n) continue;
-    const uint32_t d = (key[u] >> a.shift) & a.mask;
-    const uint32_t pos = start[d] + mine[d] + rank[u];
+  for (int u = 0; u < kTileItems; ++u)
+    if (digit[u] != 0xffffffffu)
+      stage[local[digit[u]] + mine[digit[u]] + rank[u]] = (digit[u] << 16) | static_cast<uint32_t>(first + u * 32);
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x)
+    start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] - local[c];
+  __syncthreads();
+  const int here = static_cast<int>(min(static_cast<int64_t>(kTile), a.n - tile));
+  for (int l = threadIdx.x; l < here; l += blockDim.x) {
+    const uint32_t w = stage[l], d = w >> 16;
+    const int64_t s = tile + (w & 0xffffu);
+    const uint32_t pos = start[d] + l;
+    const uint32_t key = load_key<TL, FIRST>(in, s, a.k);
     const uint32_t slot = FIRST ? static_cast<uint32_t>(s) : in_slots[s];
     if (LAST) {
-      const bool kept = key[u] < a.k;
+      const bool kept = key < a.k;
       o.order[pos] = kept ? static_cast<int32_t>(slot) : -1;
-      o.labels[pos] = kept ? static_cast<int32_t>(key[u]) : -1;
+      o.labels[pos] = kept ? static_cast<int32_t>(key) : -1;
       o.position[slot] = kept ? static_cast<int32_t>(pos) : -1;
     } else {
-      o.keys[pos] = key[u];
+      o.keys[pos] = key;
       o.slots[pos] = slot;
     }
   }
@@ -204,11 +349,13 @@ static inline size_t al(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct SortPlan {
   int passes, bits, bins, tiles;
+  bool cluster;
 };
 
 static SortPlan sort_plan(int64_t n, int64_t k) {
   SortPlan p{};
-  p.tiles = static_cast<int>((n + kTile - 1) / kTile);
+  p.cluster = n <= kClusterSlots;
+  p.tiles = static_cast<int>(((n + kTile - 1) / kTile + 3) / 4 * 4);
   if (k + 1 <= kMaxBins) {
     p.passes = 1;
     p.bins = static_cast<int>(k + 1);
@@ -216,7 +363,7 @@ static SortPlan sort_plan(int64_t n, int64_t k) {
   }
   int bits = 1;
   while ((1ll << bits) <= k) ++bits;  // keys 0 .. k
-  p.passes = (bits + 11) / 12;
+  p.passes = (bits + kPassBits - 1) / kPassBits;
   p.bits = (bits + p.passes - 1) / p.passes;
   p.bins = 1 << p.bits;
   return p;
@@ -225,25 +372,55 @@ static SortPlan sort_plan(int64_t n, int64_t k) {
 size_t group_ws_bytes(int64_t n, int64_t k) {
   if (n <= 0) return 0;
   const SortPlan p = sort_plan(n, k);
-  size_t b = al(static_cast<size_t>(p.bins) * p.tiles * 4) + al(static_cast<size_t>(p.bins) * 4);
+  size_t b = 256;
+  if (!p.cluster) b += al(static_cast<size_t>(p.bins) * p.tiles * 4) + al(static_cast<size_t>(p.bins) * 4);
   if (p.passes > 1) b += 2 * al(static_cast<size_t>(n) * 4);
   if (p.passes > 2) b += 2 * al(static_cast<size_t>(n) * 4);
   return b;
 }
 
+static cudaError_t more_smem(const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
+template <typename TL, int ITEMS>
+static cudaError_t sort_cluster(const TL* in, ClusterSort a, const SortOut& o, cudaStream_t st) {
+  // blocks of 1024 threads, as many as hold the slots; one block no larger than the slots
+  int64_t threads = (a.n + ITEMS - 1) / ITEMS;
+  int cluster = 1;
+  while (static_cast<int64_t>(cluster) * 1024 < threads) {
+    cluster *= 2;
+    ++a.log_cluster;
+  }
+  const int nt = cluster > 1 ? 1024 : static_cast<int>((threads + 31) / 32 * 32);
+  const size_t smem = static_cast<size_t>(a.bins) * (12 + 2 * (nt / 32));
+  cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_cluster_kernel<TL, ITEMS>), smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+  cfg.blockDim = dim3(static_cast<unsigned>(nt));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<TL, ITEMS>, in, a, o);
+}
+
 template <typename TL, bool FIRST, bool LAST>
 static cudaError_t sort_pass(const TL* in, const uint32_t* in_slots, const SortPass& a, const SortOut& o,
                              cudaStream_t st) {
-  const size_t hist_sm = static_cast<size_t>(a.bins) * 4;
-  const size_t sm = static_cast<size_t>(a.bins) * (4 + 2 * kSortWarps);
-  cudaError_t e = cudaSuccess;
-  if (sm > 48 * 1024)
-    e = cudaFuncSetAttribute(sort_scatter_kernel<TL, FIRST, LAST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(sm));
+  const size_t sm = static_cast<size_t>(a.bins) * (8 + 2 * kTileWarps) + kTile * 4;
+  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_scatter_kernel<TL, FIRST, LAST>), sm);
   if (e != cudaSuccess) return e;
-  sort_hist_kernel<TL><<<a.tiles, kSortWarps * 32, hist_sm, st>>>(in, a);
+  const unsigned tiles = static_cast<unsigned>((a.n + kTile - 1) / kTile);
+  sort_hist_kernel<TL, FIRST><<<tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st>>>(in, a);
   sort_tiles_kernel<<<(a.bins + 7) / 8, 256, 0, st>>>(a);
-  sort_scatter_kernel<TL, FIRST, LAST><<<a.tiles, kSortWarps * 32, sm, st>>>(in, in_slots, a, o);
+  sort_scatter_kernel<TL, FIRST, LAST><<<tiles, kTileWarps * 32, sm, st>>>(in, in_slots, a, o);
   return cudaGetLastError();
 }
 
@@ -251,48 +428,62 @@ template <typename TL>
 static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offsets, int32_t* order, int32_t* position,
                            int32_t* sorted, uint8_t* ws, cudaStream_t st) {
   const SortPlan p = sort_plan(n, k);
-  SortPass a{};
-  a.n = n;
-  a.k = static_cast<uint32_t>(k);
-  a.bins = p.bins;
-  a.tiles = p.tiles;
-  a.T = reinterpret_cast<uint32_t*>(ws);
-  ws += al(static_cast<size_t>(p.bins) * p.tiles * 4);
-  a.total = reinterpret_cast<uint32_t*>(ws);
-  ws += al(static_cast<size_t>(p.bins) * 4);
   SortOut o{};
   o.order = order;
   o.position = position;
   o.labels = sorted;
-  if (p.passes == 1) {
-    a.mask = 0xffffffffu;
-    o.offsets = offsets;
-    return sort_pass<TL, true, true>(labels, nullptr, a, o, st);
-  }
-  uint32_t* buf[4];
+  o.offsets = p.passes == 1 ? offsets : nullptr;
+  uint32_t* buf[4] = {nullptr, nullptr, nullptr, nullptr};
   for (int i = 0; i < 2 * std::min(p.passes - 1, 2); ++i) {
     buf[i] = reinterpret_cast<uint32_t*>(ws);
     ws += al(static_cast<size_t>(n) * 4);
   }
-  a.mask = static_cast<uint32_t>(p.bins - 1);
-  o.keys = buf[0];
-  o.slots = buf[1];
-  cudaError_t e = sort_pass<TL, true, false>(labels, nullptr, a, o, st);
-  const uint32_t *keys = buf[0], *slots = buf[1];
-  if (e == cudaSuccess && p.passes == 3) {
-    a.shift = p.bits;
-    o.keys = buf[2];
-    o.slots = buf[3];
-    e = sort_pass<uint32_t, false, false>(keys, slots, a, o, st);
-    keys = buf[2];
-    slots = buf[3];
+  cudaError_t e = cudaSuccess;
+  if (p.cluster) {
+    ClusterSort a{};
+    a.n = n;
+    a.k = static_cast<uint32_t>(k);
+    a.passes = p.passes;
+    a.bits = p.bits;
+    a.bins = p.bins;
+    for (int i = 0; i < 2; ++i) {
+      a.keys[i] = buf[2 * i];
+      a.slots[i] = buf[2 * i + 1];
+    }
+    e = n <= 8 * 1024 ? sort_cluster<TL, 1>(labels, a, o, st) : sort_cluster<TL, kClusterItems>(labels, a, o, st);
+  } else {
+    SortPass a{};
+    a.n = n;
+    a.k = static_cast<uint32_t>(k);
+    a.bins = p.bins;
+    a.tiles = p.tiles;
+    a.T = reinterpret_cast<uint32_t*>(ws);
+    a.total = reinterpret_cast<uint32_t*>(ws + al(static_cast<size_t>(p.bins) * p.tiles * 4));
+    if (p.passes == 1) {
+      a.mask = 0xffffffffu;
+      return sort_pass<TL, true, true>(labels, nullptr, a, o, st);
+    }
+    a.mask = static_cast<uint32_t>(p.bins - 1);
+    o.keys = buf[0];
+    o.slots = buf[1];
+    e = sort_pass<TL, true, false>(labels, nullptr, a, o, st);
+    const uint32_t *keys = buf[0], *slots = buf[1];
+    if (e == cudaSuccess && p.passes == 3) {
+      a.shift = p.bits;
+      o.keys = buf[2];
+      o.slots = buf[3];
+      e = sort_pass<uint32_t, false, false>(keys, slots, a, o, st);
+      keys = buf[2];
+      slots = buf[3];
+    }
+    a.shift = p.bits * (p.passes - 1);
+    if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(keys, slots, a, o, st);
   }
-  if (e != cudaSuccess) return e;
-  a.shift = p.bits * (p.passes - 1);
-  e = sort_pass<uint32_t, false, true>(keys, slots, a, o, st);
-  if (e != cudaSuccess) return e;
-  sort_offsets_kernel<<<static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st>>>(sorted, n, k, offsets);
-  return cudaGetLastError();
+  if (e == cudaSuccess && p.passes > 1) {
+    sort_offsets_kernel<<<static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st>>>(sorted, n, k, offsets);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 cudaError_t launch_group_rows(const void* labels, bool labels_i64, int64_t n, int64_t k, int32_t* offsets,
@@ -304,70 +495,120 @@ cudaError_t launch_group_rows(const void* labels, bool labels_i64, int64_t n, in
 }
 
 // ------------------------------------------------------------------ rows there
-// One thread per vector of a row: the vector is read once and stored at each of the row's
-// kept positions.  Rows [n, n + n p) of the walk are the output's own rows, of which those
-// behind the last kept slot are set to zero.
+// A vector of a row is read once and stored at each of the row's kept positions.  The output's
+// rows behind the last kept slot are set to zero by the grid's last blocks.
 template <typename R>
+__device__ __forceinline__ void zero_rows(R* Y, int64_t filled, int64_t slots, int64_t nv, int64_t block, int64_t blocks) {
+  const int64_t first = max(static_cast<int64_t>(0), min(filled, slots)) * nv, end = slots * nv;
+  for (int64_t f = first + block * blockDim.x + threadIdx.x; f < end; f += blocks * blockDim.x)
+    store_once(Y + f, raw_zero<R>());
+}
+
+template <typename R, int U, bool WIDE>
 __global__ void __launch_bounds__(256) rows_to_groups_kernel(const R* __restrict__ X,
                                                              const int32_t* __restrict__ position,
                                                              const int32_t* __restrict__ kept, int64_t n, int p,
-                                                             int64_t nv, R* __restrict__ Y) {
+                                                             int64_t nv, int64_t chunks, int64_t copy_blocks,
+                                                             R* __restrict__ Y) {
   const int64_t slots = n * p;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  RowWalk w(first, step, nv);
-  for (; w.row < n; w.next()) {
-    const R v = load_once(X + w.row * nv + w.v);
-    const int32_t* pos = position + w.row * p;
-    for (int j = 0; j < p; ++j) {
-      const int64_t r = pos[j];
-      if (r >= 0 && r < slots) store_once(Y + r * nv + w.v, v);
-    }
+  if (static_cast<int64_t>(blockIdx.x) >= copy_blocks) {
+    zero_rows(Y, *kept, slots, nv, blockIdx.x - copy_blocks, gridDim.x - copy_blocks);
+    return;
   }
-  const int64_t filled = max(0, *kept);
-  if (filled >= slots) return;
-  RowWalk z(first, step, nv);
-  for (; z.row + filled < slots; z.next()) store_once(Y + (z.row + filled) * nv + z.v, raw_zero<R>());
+  R x[U];
+  if constexpr (WIDE) {
+    const WideRows<1, U> w(chunks);
+    if (w.row >= n) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (w.v + 32 * u < nv) x[u] = load_once(X + w.row * nv + w.v + 32 * u);
+    for (int j = 0; j < p; ++j) {
+      const int64_t r = position[w.row * p + j];
+      if (r < 0 || r >= slots) continue;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (w.v + 32 * u < nv) store_once(Y + r * nv + w.v + 32 * u, x[u]);
+    }
+  } else {
+    const NarrowRows<U> w(nv);
+    int64_t row[U];
+    uint32_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w.at(u, row[u], v[u]);
+      if (row[u] < n) x[u] = load_once(X + row[u] * nv + v[u]);
+    }
+    for (int j = 0; j < p; ++j)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = row[u] < n ? position[row[u] * p + j] : -1;
+        if (r >= 0 && r < slots) store_once(Y + r * nv + v[u], x[u]);
+      }
+  }
 }
 
 // ------------------------------------------------------------------ rows back
-// One thread per vector of an output row, the p vectors it sums in order of j; slots that
-// were dropped (position -1) add nothing.
-template <typename T, int N, bool WEIGHTED>
+// A vector of an output row is the sum, in order of j, of the row's p vectors, J of them in
+// flight for each of the lane's U output vectors; slots that were dropped (position -1) add
+// nothing.
+template <typename T, int N, int J, int U, bool WEIGHTED, bool WIDE>
 __global__ void __launch_bounds__(256) rows_from_groups_kernel(const T* __restrict__ Z,
                                                                const int32_t* __restrict__ position,
                                                                const Acc<T>* __restrict__ weights, int64_t n, int p,
-                                                               int64_t nv, T* __restrict__ out) {
+                                                               int64_t nv, int64_t chunks, T* __restrict__ out) {
   using A = Acc<T>;
   using V = Vec<T, N>;
+  using Raw = typename V::Raw;
+  static_assert(WIDE || U == 1, "a narrow row's vector has a row of its own");
+  const Raw* Zr = reinterpret_cast<const Raw*>(Z);
   const int64_t slots = n * p;
-  const typename V::Raw* Zr = reinterpret_cast<const typename V::Raw*>(Z);
-  RowWalk w(static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<int64_t>(gridDim.x) * blockDim.x,
-            nv);
-  for (; w.row < n; w.next()) {
-    A acc[N];
+  int64_t row, v;
+  if constexpr (WIDE) {
+    const WideRows<1, U> w(chunks);
+    row = w.row;
+    v = w.v;
+  } else {
+    uint32_t at;
+    NarrowRows<1>(nv).at(0, row, at);
+    v = at;
+  }
+  if (row >= n) return;
+  const int32_t* pos = position + row * p;
+  const A* wts = WEIGHTED ? weights + row * p : nullptr;
+  A acc[U][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = A(0);
-    const int32_t* pos = position + w.row * p;
-    for (int j0 = 0; j0 < p; j0 += 4) {
-      V z[4];
-      A wt[4];
+  for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t r = j0 + u < p ? pos[j0 + u] : -1;
-        const bool ok = r >= 0 && r < slots;
-        z[u].raw = ok ? load_once(Zr + r * nv + w.v) : raw_zero<typename V::Raw>();
-        wt[u] = ok ? (WEIGHTED ? weights[w.row * p + j0 + u] : A(1)) : A(0);
+    for (int e = 0; e < N; ++e) acc[u][e] = A(0);
+  for (int j0 = 0; j0 < p; j0 += J) {
+    V z[J][U];
+    A wt[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int64_t r = j0 + j < p ? pos[j0 + j] : -1;
+      const bool ok = r >= 0 && r < slots;
+      wt[j] = WEIGHTED && j0 + j < p ? wts[j0 + j] : A(1);
+      wt[j] = ok ? wt[j] : A(0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        z[j][u].raw = raw_zero<Raw>();
+        if (ok && v + 32 * u < nv) z[j][u].raw = load_once(Zr + r * nv + v + 32 * u);
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += wt[u] * to_acc(z[u].e[e]);
     }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[u][e] += wt[j] * to_acc(z[j][u].e[e]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (v + 32 * u >= nv) continue;
     V o;
 #pragma unroll
-    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(acc[e]);
-    store_once(reinterpret_cast<typename V::Raw*>(out) + w.row * nv + w.v, o.raw);
+    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(acc[u][e]);
+    store_once(reinterpret_cast<Raw*>(out) + row * nv + v + 32 * u, o.raw);
   }
 }
 
@@ -384,6 +625,7 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
   using V = Vec<T, N>;
   using Raw = typename V::Raw;
   constexpr int TEAMS = 8 / TEAM_WARPS;
+  constexpr int UV = N * sizeof(T) >= 16 ? 1 : N * sizeof(T) == 8 ? 2 : 4;  // vectors in flight, with each pick's
   __shared__ A part[8][4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int team = warp / TEAM_WARPS, in_team = threadIdx.x - team * TEAM_WARPS * 32;
@@ -405,28 +647,42 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
           if (r[u] >= slots) r[u] = -1;
           wt[u] = r[u] >= 0 ? (weights ? weights[i * p + j0 + u] : A(1)) : A(0);
         }
-        for (int64_t v = in_team; v < nv; v += TEAM_WARPS * 32) {
-          V g, z[4];
-          g.raw = load_keep(Gr + i * nv + v);
-          if (gW) {
+        for (int64_t v0 = in_team; v0 < nv; v0 += UV * TEAM_WARPS * 32) {
+          V g[UV], z[UV][4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              z[u].raw = r[u] >= 0 ? load_once(Zr + r[u] * nv + v) : raw_zero<Raw>();
+          for (int q = 0; q < UV; ++q) {
+            const int64_t v = v0 + q * (TEAM_WARPS * 32);
+            g[q].raw = raw_zero<Raw>();
+            if (v < nv) g[q].raw = load_keep(Gr + i * nv + v);
+            if (gW) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                z[q][u].raw = raw_zero<Raw>();
+                if (r[u] >= 0 && v < nv) z[q][u].raw = load_once(Zr + r[u] * nv + v);
+              }
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < UV; ++q) {
+            const int64_t v = v0 + q * (TEAM_WARPS * 32);
+            if (v >= nv) continue;
+            if (gW) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (r[u] >= 0) {
+#pragma unroll
+                  for (int e = 0; e < N; ++e) dot[u] += to_acc(g[q].e[e]) * to_acc(z[q][u].e[e]);
+                }
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
               if (r[u] >= 0) {
+                V o;
 #pragma unroll
-                for (int e = 0; e < N; ++e) dot[u] += to_acc(g.e[e]) * to_acc(z[u].e[e]);
+                for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(wt[u] * to_acc(g[q].e[e]));
+                store_once(gZr + r[u] * nv + v, o.raw);
               }
           }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (r[u] >= 0) {
-              V o;
-#pragma unroll
-              for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(wt[u] * to_acc(g.e[e]));
-              store_once(gZr + r[u] * nv + v, o.raw);
-            }
         }
       }
       if (gW) {
@@ -455,26 +711,40 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
       }
     }
   }
-  const int64_t filled = max(0, *kept);
-  if (filled >= slots) return;
-  RowWalk z(static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<int64_t>(gridDim.x) * blockDim.x,
-            nv);
-  for (; z.row + filled < slots; z.next()) store_once(gZr + (z.row + filled) * nv + z.v, raw_zero<Raw>());
+  zero_rows(gZr, *kept, slots, nv, blockIdx.x, gridDim.x);
 }
 
 // ------------------------------------------------------------------ launches
-static unsigned grid_for(int64_t items, int per_block, int waves) {
-  const int64_t most = static_cast<int64_t>(num_sms()) * waves;
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((items + per_block - 1) / per_block, most)));
+// Blocks that clear the rows behind the last kept slot (how many there are is known on the
+// device alone): enough to write at HBM's rate, and gone at once where there are none.
+static int64_t clear_blocks(int64_t vectors) {
+  return std::min<int64_t>((vectors + 255) / 256, static_cast<int64_t>(num_sms()) * 4);
 }
 
+template <typename R, int U>
+static cudaError_t to_groups_u(const R* X, const int32_t* position, const int32_t* kept, int64_t n, int p, int64_t nv,
+                               R* Y, cudaStream_t st) {
+  const bool wide = nv >= 32;
+  const int64_t chunks = (nv + 32 * U - 1) / (32 * U);
+  const int64_t copy = wide ? wide_blocks(n, nv, 1, U) : narrow_blocks(n, nv, U);
+  const unsigned g = static_cast<unsigned>(copy + clear_blocks(n * p * nv));
+  if (wide)
+    rows_to_groups_kernel<R, U, true><<<g, 256, 0, st>>>(X, position, kept, n, p, nv, chunks, copy, Y);
+  else
+    rows_to_groups_kernel<R, U, false><<<g, 256, 0, st>>>(X, position, kept, n, p, nv, chunks, copy, Y);
+  return cudaGetLastError();
+}
+
+// Four vectors a lane in flight, eight narrow ones; fewer where the row has no more.
 template <typename R>
 static cudaError_t to_groups_t(const void* X, const int32_t* position, const int32_t* kept, int64_t n, int p,
                                int64_t row_bytes, void* Y, cudaStream_t st) {
   const int64_t nv = row_bytes / static_cast<int64_t>(sizeof(R));
-  rows_to_groups_kernel<R><<<grid_for(n * nv, 256, 64), 256, 0, st>>>(static_cast<const R*>(X), position, kept, n, p,
-                                                                      nv, static_cast<R*>(Y));
-  return cudaGetLastError();
+  const R* x = static_cast<const R*>(X);
+  R* y = static_cast<R*>(Y);
+  if (nv >= 32 && nv <= 64) return to_groups_u<R, 2>(x, position, kept, n, p, nv, y, st);
+  if (sizeof(R) >= 8 || nv < 256) return to_groups_u<R, 4>(x, position, kept, n, p, nv, y, st);
+  return to_groups_u<R, 8>(x, position, kept, n, p, nv, y, st);
 }
 
 cudaError_t launch_rows_to_groups(int esize, const void* X, const int32_t* position, const int32_t* kept, int64_t n,
@@ -488,17 +758,33 @@ cudaError_t launch_rows_to_groups(int esize, const void* X, const int32_t* posit
   }
 }
 
+template <typename T, int N, int J, bool WEIGHTED>
+static cudaError_t from_groups_j(const T* Z, const int32_t* position, const Acc<T>* w, int64_t n, int p, int64_t nv,
+                                 T* out, cudaStream_t st) {
+  constexpr int U = N * sizeof(T) >= 8 ? 1 : 4;
+  if (nv >= 32)
+    rows_from_groups_kernel<T, N, J, U, WEIGHTED, true><<<static_cast<unsigned>(wide_blocks(n, nv, 1, U)), 256, 0, st>>>(
+        Z, position, w, n, p, nv, (nv + 32 * U - 1) / (32 * U), out);
+  else
+    rows_from_groups_kernel<T, N, J, 1, WEIGHTED, false><<<static_cast<unsigned>(narrow_blocks(n, nv, 1)), 256, 0, st>>>(
+        Z, position, w, n, p, nv, 1, out);
+  return cudaGetLastError();
+}
+
+template <typename T, int N, bool WEIGHTED>
+static cudaError_t from_groups_w(const T* Z, const int32_t* position, const Acc<T>* w, int64_t n, int p, int64_t nv,
+                                 T* out, cudaStream_t st) {
+  if (p <= 2) return from_groups_j<T, N, 2, WEIGHTED>(Z, position, w, n, p, nv, out, st);
+  if (p <= 4) return from_groups_j<T, N, 4, WEIGHTED>(Z, position, w, n, p, nv, out, st);
+  return from_groups_j<T, N, 8, WEIGHTED>(Z, position, w, n, p, nv, out, st);
+}
+
 template <typename T, int N>
 static cudaError_t from_groups_n(const T* Z, const int32_t* position, const void* weights, int64_t n, int p,
                                  int64_t dim, T* out, cudaStream_t st) {
-  const int64_t nv = dim / N;
-  const unsigned g = grid_for(n * nv, 256, 64);
   const Acc<T>* w = static_cast<const Acc<T>*>(weights);
-  if (w)
-    rows_from_groups_kernel<T, N, true><<<g, 256, 0, st>>>(Z, position, w, n, p, nv, out);
-  else
-    rows_from_groups_kernel<T, N, false><<<g, 256, 0, st>>>(Z, position, w, n, p, nv, out);
-  return cudaGetLastError();
+  return w ? from_groups_w<T, N, true>(Z, position, w, n, p, dim / N, out, st)
+           : from_groups_w<T, N, false>(Z, position, w, n, p, dim / N, out, st);
 }
 
 template <typename T, int N>
@@ -508,12 +794,14 @@ static cudaError_t from_groups_grad_n(const T* G, const T* Z, const int32_t* pos
   const int64_t nv = dim / N;
   const Acc<T>* w = static_cast<const Acc<T>*>(weights);
   Acc<T>* gw = static_cast<Acc<T>*>(gW);
+  const int64_t most = static_cast<int64_t>(num_sms()) * 64;
+  // a block per row, for what it has in flight; a warp where the row is no longer than that
   if (nv <= 64)
-    rows_from_groups_grad_kernel<T, N, 1>
-        <<<grid_for(n, 8, 64), 256, 0, st>>>(G, Z, position, w, kept, n, p, nv, gZ, gw);
+    rows_from_groups_grad_kernel<T, N, 1><<<static_cast<unsigned>(std::min<int64_t>((n + 7) / 8, most)), 256, 0, st>>>(
+        G, Z, position, w, kept, n, p, nv, gZ, gw);
   else
-    rows_from_groups_grad_kernel<T, N, 8>
-        <<<grid_for(n, 1, 64), 256, 0, st>>>(G, Z, position, w, kept, n, p, nv, gZ, gw);
+    rows_from_groups_grad_kernel<T, N, 8><<<static_cast<unsigned>(std::min<int64_t>(n, most)), 256, 0, st>>>(
+        G, Z, position, w, kept, n, p, nv, gZ, gw);
   return cudaGetLastError();
 }
 

@@ -62,30 +62,50 @@ inline int row_vec_bytes(int64_t row_bytes, uintptr_t addresses) {
   return (a & 15u) == 0 ? 16 : (a & 7u) == 0 ? 8 : (a & 3u) == 0 ? 4 : 2;
 }
 
-// A walk over the vectors of consecutive rows, one vector of a row per thread: the flat
-// index is split into (row, vector) by one division at the start, and a step of `step`
-// vectors adds the step's own (rows, vectors) with a carry.
-struct RowWalk {
-  int64_t row;
-  int64_t v;
-  int64_t step_rows;
-  int64_t step_v;
-  int64_t nv;
-  __device__ __forceinline__ RowWalk(int64_t first, int64_t step, int64_t nv_) : nv(nv_) {
-    row = first / nv;
-    v = first - row * nv;
-    step_rows = step / nv;
-    step_v = step - step_rows * nv;
-  }
-  __device__ __forceinline__ void next() {
-    row += step_rows;
-    v += step_v;
-    if (v >= nv) {
-      v -= nv;
-      ++row;
+// How the row kernels cut rows of nv vectors into work (kUnit threads' worth a block).
+//
+// Wide rows (nv >= 32): a warp takes R neighbouring rows times a chunk of 32 U vectors, so a
+// row's number and what goes with it (label, position) are the warp's own, and R U vectors a
+// lane are in flight.  Narrow rows: a block takes 256 U consecutive vectors of the matrix,
+// each thread those at a stride of 256, and finds every vector's row by a 32-bit division.
+// Either way neighbouring lanes hold neighbouring vectors.
+template <int R, int U> struct WideRows {
+  int64_t row;  // the first of the warp's R rows
+  int64_t v;    // this lane's first vector; the u-th is v + 32 u
+  __device__ __forceinline__ WideRows(int64_t chunks) {
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    int64_t group;
+    if (unit < 0x80000000ll && chunks < 0x80000000ll) {
+      group = static_cast<uint32_t>(unit) / static_cast<uint32_t>(chunks);
+    } else {
+      group = unit / chunks;
     }
+    row = group * R;
+    v = (unit - group * chunks) * (32 * U) + (threadIdx.x & 31);
   }
 };
+template <int U> struct NarrowRows {
+  int64_t row0;
+  uint32_t rest, nv;
+  __device__ __forceinline__ NarrowRows(int64_t nv_) : nv(static_cast<uint32_t>(nv_)) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 * U);
+    row0 = first < 0x80000000ll ? static_cast<int64_t>(static_cast<uint32_t>(first) / nv) : first / nv_;
+    rest = static_cast<uint32_t>(first - row0 * nv_) + threadIdx.x;
+  }
+  // row and vector of this thread's u-th
+  __device__ __forceinline__ void at(int u, int64_t& row, uint32_t& v) const {
+    const uint32_t f = rest + 256u * u, q = f / nv;
+    row = row0 + q;
+    v = f - q * nv;
+  }
+};
+
+// blocks of 256 threads for `rows` rows of nv vectors
+inline int64_t wide_blocks(int64_t rows, int64_t nv, int R, int U) {
+  const int64_t chunks = (nv + 32 * U - 1) / (32 * U);
+  return ((rows + R - 1) / R * chunks + 7) / 8;
+}
+inline int64_t narrow_blocks(int64_t rows, int64_t nv, int U) { return (rows * nv + 256 * U - 1) / (256 * U); }
 
 // Calls F<T, N>(...) for the widest vector of N elements that `bytes` allows.
 #define EUC_ROW_VEC(T, bytes, F, ...)                                                    \
