@@ -139,8 +139,19 @@ def ptr(t):
 def call_on(t, fn, *args):
     """fn(*args, stream) on t's device and its current stream, the caller's current device
     left as it was; tensors are passed as addresses (data_ptr(), None for absent ones)."""
-    with torch.cuda.device(t.device):
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    d = t.get_device()
+    if torch.cuda.current_device() == d:
+        rc = fn(*args, _raw_stream(d))
+    else:
+        with torch.cuda.device(d):
+            rc = fn(*args, _raw_stream(d))
+    if rc:
+        check(rc)
+
+
+# the current stream's handle without a Stream object around it (3 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
 def workspace(nbytes, device):

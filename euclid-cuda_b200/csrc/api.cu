@@ -96,9 +96,14 @@ int device_error_and_clear() {
 }
 
 bool device_is_sm100() {
+  static std::atomic<int> known[64];  // major compute capability per device, 0: not asked yet
   int dev = 0, major = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return false;
+  if (dev >= 0 && dev < 64) major = known[dev].load(std::memory_order_relaxed);
+  if (major == 0) {
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return false;
+    if (dev >= 0 && dev < 64) known[dev].store(major, std::memory_order_relaxed);
+  }
   return major == 10;
 }
 

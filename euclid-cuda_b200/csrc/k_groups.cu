@@ -372,7 +372,7 @@ static SortPlan sort_plan(int64_t n, int64_t k) {
 size_t group_ws_bytes(int64_t n, int64_t k) {
   if (n <= 0) return 0;
   const SortPlan p = sort_plan(n, k);
-  size_t b = 256;
+  size_t b = 0;
   if (!p.cluster) b += al(static_cast<size_t>(p.bins) * p.tiles * 4) + al(static_cast<size_t>(p.bins) * 4);
   if (p.passes > 1) b += 2 * al(static_cast<size_t>(n) * 4);
   if (p.passes > 2) b += 2 * al(static_cast<size_t>(n) * 4);

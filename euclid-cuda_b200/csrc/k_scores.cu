@@ -975,9 +975,11 @@ template <typename T, int NT> static cudaError_t scores_block(const ScoreArgs<T>
   const int per_group = static_cast<int>(std::max<int64_t>(1, (steps + kGroups - 1) / kGroups));
   const size_t groups = static_cast<size_t>((steps + per_group - 1) / per_group);
   const size_t smem = a.top ? groups * NT * sizeof(Acc<T>) : 0;
-  cudaError_t e = cudaFuncSetAttribute(scores_block_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kGroups * NT * sizeof(Acc<T>)));
-  if (e != cudaSuccess) return e;
+  if (smem > 32 * 1024) {  // beyond 48 KiB with the static arrays
+    const cudaError_t e = cudaFuncSetAttribute(scores_block_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(kGroups * NT * sizeof(Acc<T>)));
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.n * cluster));
   cfg.blockDim = dim3(NT);

@@ -123,7 +123,7 @@ int euc_group_rows(const void* labels, int labels_are_i64, int64_t slots, int64_
   if (!offsets || (slots > 0 && (!labels || !order || !position || !sorted_labels)))
     return set_error(EUC_ERR_ARG, "null pointer");
   const size_t need = group_ws_bytes(slots, k);
-  if (slots > 0 && (!ws || ws_bytes < need))
+  if (need > 0 && (!ws || ws_bytes < need))
     return set_error(EUC_ERR_WORKSPACE, ("group_rows: workspace of " + std::to_string(need) + " bytes required").c_str());
   return done(launch_group_rows(labels, labels_are_i64 != 0, slots, k, offsets, order, position, sorted_labels, ws,
                                 static_cast<cudaStream_t>(stream)),

@@ -56,9 +56,10 @@ def group_rows(labels, n_clusters):
     order = torch.empty(slots, dtype=torch.int32, device=dev)
     position = torch.empty(labels.shape, dtype=torch.int32, device=dev)
     sorted_labels = torch.empty(slots, dtype=torch.int32, device=dev)
-    ws = workspace(lib().euc_group_rows_workspace_bytes(slots, k), dev)
+    need = lib().euc_group_rows_workspace_bytes(slots, k)
+    ws = workspace(need, dev) if need else None
     call_on(labels, lib().euc_group_rows, labels.data_ptr(), i64, slots, k, offsets.data_ptr(), order.data_ptr(),
-            position.data_ptr(), sorted_labels.data_ptr(), ws.data_ptr(), ws.numel())
+            position.data_ptr(), sorted_labels.data_ptr(), ws.data_ptr() if need else None, need)
     return RowGroups(offsets, order, position, sorted_labels)
 
 
@@ -66,13 +67,14 @@ def check_groups(groups):
     """A RowGroups whose parts fit together (their values are checked by the kernels)."""
     if not isinstance(groups, RowGroups):
         raise TypeError("groups must be a RowGroups")
-    for t, name in zip(groups, RowGroups._fields):
-        _ops.check_input(t, "groups." + name)
-        if t.dtype != torch.int32 or t.device != groups.offsets.device:
+    offsets, order, position, labels = groups
+    for t, name in ((offsets, "offsets"), (order, "order"), (position, "position"), (labels, "labels")):
+        _ops.check_input(t, name)
+        if t.dtype != torch.int32 or t.get_device() != offsets.get_device():
             raise RuntimeError(f"groups.{name} must be int32 on the groups' device")
-    slots = groups.position.numel()
-    if groups.offsets.dim() != 1 or groups.offsets.numel() < 1 or groups.position.dim() not in (1, 2) or \
-            groups.order.numel() != slots or groups.labels.numel() != slots:
+    slots = position.numel()
+    if offsets.dim() != 1 or offsets.numel() < 1 or position.dim() not in (1, 2) or \
+            order.numel() != slots or labels.numel() != slots:
         raise RuntimeError("groups do not fit together")
 
 

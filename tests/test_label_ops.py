@@ -91,7 +91,11 @@ def test_groups_abi_checks(lib):
     big = 2 ** 31 - 1
     assert lib.euc_group_rows_workspace_bytes(0, 5) == 0
     assert lib.euc_group_rows_workspace_bytes(big, 5) == 0 and lib.euc_group_rows_workspace_bytes(5, big) == 0
-    assert lib.euc_group_rows_workspace_bytes(1000, 64) > 0
+    # one cluster, one pass: none; several passes keep keys and slots between them; many slots
+    # keep a histogram per tile too
+    assert lib.euc_group_rows_workspace_bytes(1000, 64) == 0
+    assert lib.euc_group_rows_workspace_bytes(1000, 100000) >= 2 * 4000
+    assert lib.euc_group_rows_workspace_bytes(1 << 20, 64) >= 65 * 512 * 4
     f = lib.euc_group_rows
     assert f(P, 1, -1, 4, P, P, P, P, P, 1 << 20, None) == 1 and f(P, 1, 4, -1, P, P, P, P, P, 1 << 20, None) == 1
     assert f(P, 1, big, 4, P, P, P, P, P, 1 << 20, None) == 1 and f(P, 1, 4, big, P, P, P, P, P, 1 << 20, None) == 1
@@ -103,7 +107,7 @@ def test_groups_abi_checks(lib):
         assert f(P, 1, 4, 4, P, P, P, P, P, 1 << 20, None) == 8 and t(0, P, P, P, 4, 2, 8, P, None) == 8
         assert b(0, P, P, P, 4, 2, 8, P, None) == 8 and g(0, P, P, P, P, P, 4, 2, 8, P, P, None) == 8
     else:
-        assert f(P, 1, 4, 4, P, P, P, P, P, 16, None) == 6      # EUC_ERR_WORKSPACE
+        assert f(P, 1, 4, 10000, P, P, P, P, P, 16, None) == 6      # EUC_ERR_WORKSPACE
         assert f(P, 1, 4, 4, P, None, P, P, P, 1 << 20, None) == 7
         assert t(0, None, P, P, 4, 2, 8, P, None) == 7 and b(0, P, P, P, 4, 2, 8, None, None) == 7
         assert t(0, ctypes.c_void_p(258), P, P, 4, 2, 8, P, None) == 7
