@@ -84,12 +84,16 @@ struct GradArgs {
   int64_t chunks;
 };
 
-// zero rows for the labels without rows, a warp per label and 32 vectors at a time
+// zero rows for the labels without rows: a warp takes 32 labels (whose emptiness is one
+// ballot) times a chunk of at most kClearVecs vectors
+constexpr int kClearVecs = 128;
+
 template <typename Raw>
 __device__ __forceinline__ void clear_rows(const GradArgs& a, int64_t block, int64_t blocks, Raw* out) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // 32 labels per warp: their emptiness is one ballot
-  for (int64_t c0 = (block * 8 + warp) * 32; c0 < a.k; c0 += blocks * 256) {
+  const int64_t chunks = (a.nv + kClearVecs - 1) / kClearVecs, units = (a.k + 31) / 32 * chunks;
+  for (int64_t unit = block * 8 + warp; unit < units; unit += blocks * 8) {
+    const int64_t c0 = unit / chunks * 32, v0 = unit % chunks * kClearVecs;
     const int64_t c = c0 + lane;
     const bool empty = c < a.k && a.offsets[c + 1] <= a.offsets[c];
     unsigned todo = __ballot_sync(0xffffffffu, empty);
@@ -101,7 +105,9 @@ __device__ __forceinline__ void clear_rows(const GradArgs& a, int64_t block, int
     }
     while (todo) {
       Raw* row = out + (c0 + __ffs(todo) - 1) * a.nv;
-      for (int64_t v = lane; v < a.nv; v += 32) store_once(row + v, raw_zero<Raw>());
+#pragma unroll
+      for (int u = 0; u < kClearVecs / 32; ++u)
+        if (v0 + u * 32 + lane < a.nv) store_once(row + v0 + u * 32 + lane, raw_zero<Raw>());
       todo &= todo - 1;
     }
   }
@@ -116,12 +122,24 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
   using Raw = typename V::Raw;
   const Raw* Gr = reinterpret_cast<const Raw*>(G);
   Raw* Or = reinterpret_cast<Raw*>(out);
-  if (static_cast<int64_t>(blockIdx.x) >= chunk_blocks) {
-    clear_rows<Raw>(a, blockIdx.x - chunk_blocks, gridDim.x - chunk_blocks, Or);
+  let_next_start();
+  // blocks that clear and blocks that sum take turns, so that one's writes and the other's
+  // reads overlap
+  const int64_t clear_blocks = gridDim.x - chunk_blocks, both = 2 * min(chunk_blocks, clear_blocks);
+  int64_t block = blockIdx.x;
+  bool clears = chunk_blocks < clear_blocks;
+  if (block < both) {
+    clears = block & 1;
+    block >>= 1;
+  } else {
+    block -= both / 2;
+  }
+  if (clears) {
+    clear_rows<Raw>(a, block, clear_blocks, Or);
     return;
   }
   const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t t = block * blockDim.x + threadIdx.x;
   const int64_t chunk = t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(a.nv) : t / a.nv;
   const int64_t v = t - chunk * a.nv;
   const int64_t p0 = chunk * a.seg;
@@ -177,27 +195,30 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
 }
 
 // A label that crosses chunks' borders is joined at the first border inside it: by the
-// thread of (border, vector) if it has at most kLongChunks chunks more, else by the block
+// lanes of (border, vector) if it has fewer than kLongChunks chunks more, else by the block
 // that belongs to the first multiple of kLongChunks among its chunks, whose lanes take
 // neighbouring vectors, its other threads every so-manyth chunk, and whose sums are added in
 // a fixed order.
-constexpr int kLongChunks = 16;
+constexpr int kLongChunks = 64;
+constexpr int kJoinThreads = 1024;
+constexpr int kJoinCandidates = 4;  // multiples of kLongChunks that a block looks at
 
 // sum over chunks [c, c1], every `step`-th, of the label that starts at position lo
 template <typename A, int N>
 __device__ __forceinline__ void add_parts(const A* part, int64_t c, int64_t c1, int64_t step, int64_t lo, int seg,
                                           int64_t nv, int64_t v, A* acc) {
-  for (; c <= c1; c += 4 * step) {
-    A from[4][N];
+  constexpr int P = N * sizeof(A) >= 32 ? 4 : 8;  // in flight
+  for (; c <= c1; c += P * step) {
+    A from[P][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < P; ++u) {
       const int64_t q = c + u * step;
       const A* at = part + ((2 * q + (lo < q * seg ? 0 : 1)) * nv + v) * N;
 #pragma unroll
       for (int e = 0; e < N; ++e) from[u][e] = q <= c1 ? at[e] : A(0);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < P; ++u)
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] += from[u][e];
   }
@@ -208,56 +229,80 @@ __device__ __forceinline__ void join_long(const GradArgs& a, int64_t block, Acc<
                                           const Acc<T>* __restrict__ part, T* __restrict__ out) {
   using A = Acc<T>;
   using V = Vec<T, N>;
-  __shared__ A sums[256][N];
+  __shared__ A sums[kJoinThreads][N];
+  __shared__ int owner[kJoinCandidates];  // the candidate's label, or -1
   // lanes over vectors: the power of two that holds the row, at most a warp
   int width = 32;
   while (width > 1 && width / 2 >= a.nv) width /= 2;
   const int64_t tiles = (a.nv + width - 1) / width;
-  const int64_t chunk = block / tiles * kLongChunks;
+  const int64_t first = block / tiles * kJoinCandidates;
   const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
-  if (chunk * a.seg >= total) return;
-  const int64_t c = a.labels[chunk * a.seg];
-  if (c < 0 || c >= a.k) return;
-  const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
-  if (hi <= lo) return;
-  const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
-  // (chunk's first row has the label, so the multiple before it is the only other candidate)
-  if (c1 - c0 < kLongChunks || (chunk - kLongChunks) * a.seg >= lo) return;
-  const int groups = 256 / width, group = static_cast<int>(threadIdx.x) / width, lane = static_cast<int>(threadIdx.x) % width;
-  const int64_t v = block % tiles * width + lane;
-  A acc[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = A(0);
-  if (v < a.nv) add_parts<A, N>(part, c0 + group, c1, groups, lo, a.seg, a.nv, v, acc);
-#pragma unroll
-  for (int e = 0; e < N; ++e) sums[threadIdx.x][e] = acc[e];
-  for (int half = groups / 2; half > 0; half /= 2) {
-    __syncthreads();
-    if (group < half)
-#pragma unroll
-      for (int e = 0; e < N; ++e) sums[threadIdx.x][e] += sums[threadIdx.x + half * width][e];
+  if (threadIdx.x < kJoinCandidates) {
+    const int64_t at = (first + threadIdx.x) * kLongChunks * a.seg;
+    int label = -1;
+    if (at < total) {
+      const int64_t c = a.labels[at];
+      if (c >= 0 && c < a.k) {
+        const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
+        // (the chunk's first row has the label, so the multiple before it is the only other candidate)
+        if (hi > lo && (hi - 1) / a.seg - lo / a.seg >= kLongChunks && at - static_cast<int64_t>(kLongChunks) * a.seg < lo)
+          label = static_cast<int>(c);
+      }
+    }
+    owner[threadIdx.x] = label;
   }
-  if (group == 0 && v < a.nv) {
-    V o;
+  __syncthreads();
+  const int groups = kJoinThreads / width, group = static_cast<int>(threadIdx.x) / width,
+            lane = static_cast<int>(threadIdx.x) % width;
+  const int64_t v = block % tiles * width + lane;
+  for (int q = 0; q < kJoinCandidates; ++q) {
+    const int64_t c = owner[q];
+    if (c < 0) continue;
+    const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
+    const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
+    A acc[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * sums[threadIdx.x][e]);
-    store_once(reinterpret_cast<typename V::Raw*>(out) + c * a.nv + v, o.raw);
+    for (int e = 0; e < N; ++e) acc[e] = A(0);
+    if (v < a.nv) add_parts<A, N>(part, c0 + group, c1, groups, lo, a.seg, a.nv, v, acc);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e) sums[threadIdx.x][e] = acc[e];
+    for (int half = groups / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (group < half)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sums[threadIdx.x][e] += sums[threadIdx.x + half * width][e];
+    }
+    if (group == 0 && v < a.nv) {
+      V o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * sums[threadIdx.x][e]);
+      store_once(reinterpret_cast<typename V::Raw*>(out) + c * a.nv + v, o.raw);
+    }
   }
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int64_t long_blocks, Acc<T> scale,
+template <typename T, int N, int SUB>
+__global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(GradArgs a, int64_t long_blocks, Acc<T> scale,
                                                         const Acc<T>* __restrict__ part, T* __restrict__ out) {
   using A = Acc<T>;
   using V = Vec<T, N>;
   using Raw = typename V::Raw;
+  wait_for_previous();
   if (static_cast<int64_t>(blockIdx.x) < long_blocks) {  // the longest work starts first
     join_long<T, N>(a, blockIdx.x, scale, part, out);
     return;
   }
+  // SUB 4: a warp takes eight neighbouring vectors at one border, its four lanes of a vector
+  // every fourth chunk; SUB 1 (rows of fewer vectors): a thread per vector and border
+  constexpr int VW = 32 / SUB;
+  const int lane = threadIdx.x & 31, sub = lane / VW;
   const int64_t t = static_cast<int64_t>(blockIdx.x - long_blocks) * blockDim.x + threadIdx.x;
-  const int64_t border = 1 + (t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(a.nv) : t / a.nv);
-  const int64_t v = t - (border - 1) * a.nv, at = border * a.seg;
+  const int64_t unit = SUB == 1 ? t : t >> 5, tiles = SUB == 1 ? a.nv : (a.nv + VW - 1) / VW;
+  const int64_t border =
+      1 + (unit < 0x80000000ll ? static_cast<uint32_t>(unit) / static_cast<uint32_t>(tiles) : unit / tiles);
+  const int64_t tile = unit - (border - 1) * tiles;
+  const int64_t v = SUB == 1 ? tile : tile * VW + lane % VW, at = border * a.seg;
   if (at >= min(a.n, static_cast<int64_t>(a.offsets[a.k]))) return;
   const int64_t c = a.labels[at];
   if (c < 0 || c >= a.k || a.labels[at - 1] != c) return;
@@ -267,7 +312,14 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int64_t long
   A acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = A(0);
-  add_parts<A, N>(part, c0, c1, 1, lo, a.seg, a.nv, v, acc);
+  if (v < a.nv) add_parts<A, N>(part, c0 + (SUB == 1 ? 0 : sub), c1, SUB, lo, a.seg, a.nv, v, acc);
+  if constexpr (SUB > 1) {  // (the warp is at one border: all of its lanes are here)
+#pragma unroll
+    for (int s = VW; s < 32; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], s);
+  }
+  if ((SUB > 1 && sub != 0) || v >= a.nv) return;
   V o;
 #pragma unroll
   for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
@@ -275,12 +327,12 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int64_t long
 }
 
 // ------------------------------------------------------------------ launches
-// Rows per chunk: as many as leave 32 warps per SM, since every chunk may cost two partial
+// Rows per chunk: as many as leave 16 warps per SM, since every chunk may cost two partial
 // sums and their join.  `row_bytes` / 16 stands for the row's vectors at any alignment.
 static int grad_seg(int64_t n, int64_t row_bytes) {
   const int64_t nv = std::max<int64_t>(1, row_bytes / 16);
   int seg = 16;
-  while (seg < 256 && n / (2 * seg) * nv >= static_cast<int64_t>(num_sms()) * 1024) seg *= 2;
+  while (seg < 256 && n / (2 * seg) * nv >= static_cast<int64_t>(num_sms()) * 512) seg *= 2;
   return seg;
 }
 
@@ -310,7 +362,7 @@ static cudaError_t lookup_go(const T* C, int64_t k, const TL* labels, int64_t n,
   if (n * nv <= static_cast<int64_t>(num_sms()) * 2048) return wide(lookup_kernel<T, N, TL, 1, 1, true>, 1, 1);
   if (nv <= 32) return wide(lookup_kernel<T, N, TL, 4, 1, true>, 4, 1);
   if (nv <= 64) return wide(lookup_kernel<T, N, TL, 2, 2, true>, 2, 2);
-  return wide(lookup_kernel<T, N, TL, 1, 4, true>, 1, 4);
+  return wide(lookup_kernel<T, N, TL, 1, 2, true>, 1, 2);
 }
 
 template <typename T, int N>
@@ -326,15 +378,24 @@ static cudaError_t grad_n(const T* G, GradArgs a, int64_t dim, double scale, T* 
   Acc<T>* part = static_cast<Acc<T>*>(ws);
   const Acc<T> s = static_cast<Acc<T>>(scale);
   const int64_t sums = (a.chunks * a.nv + 255) / 256;
-  const int64_t clears = std::min<int64_t>((a.k + 255) / 256, static_cast<int64_t>(num_sms()) * 8);
+  const int64_t clears = std::min<int64_t>(
+      ((a.k + 31) / 32 * ((a.nv + kClearVecs - 1) / kClearVecs) + 7) / 8, static_cast<int64_t>(num_sms()) * 16);
   grad_chunks_kernel<T, N><<<static_cast<unsigned>(sums + clears), 256, 0, st>>>(G, a, sums, s, out, part);
   if (a.chunks > 1) {
     int width = 32;
     while (width > 1 && width / 2 >= a.nv) width /= 2;
     const int64_t longs =
-        a.chunks > kLongChunks ? (a.chunks + kLongChunks - 1) / kLongChunks * ((a.nv + width - 1) / width) : 0;
-    const int64_t shorts = ((a.chunks - 1) * a.nv + 255) / 256;
-    grad_join_kernel<T, N><<<static_cast<unsigned>(longs + shorts), 256, 0, st>>>(a, longs, s, part, out);
+        a.chunks > kLongChunks
+            ? (a.chunks + kLongChunks * kJoinCandidates - 1) / (kLongChunks * kJoinCandidates) * ((a.nv + width - 1) / width)
+            : 0;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // four lanes a vector where the row has eight vectors to fill the warp's others
+    const bool four = a.nv >= 8;
+    const int64_t threads = (a.chunks - 1) * (four ? (a.nv + 7) / 8 * 32 : a.nv);
+    const unsigned g = static_cast<unsigned>(longs + (threads + kJoinThreads - 1) / kJoinThreads);
+    return four ? launch_after(true, grad_join_kernel<T, N, 4>, g, kJoinThreads, 0, st, a, longs, s, part, out)
+                : launch_after(true, grad_join_kernel<T, N, 1>, g, kJoinThreads, 0, st, a, longs, s, part, out);
   }
   return cudaGetLastError();
 }

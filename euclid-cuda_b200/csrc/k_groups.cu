@@ -10,17 +10,16 @@
 //   dZ[position[i, j]] = w[i, j] dOut[i]  dw[i, j] = <dOut[i], Z[position[i, j]]>
 // and dX[i] = sum_j dY[position[i, j]], the second with weights of one.
 //
-// The sort is a counting sort in passes of up to kMaxBins bins (one pass for k < kMaxBins,
+// The sort is a counting sort in passes of up to kMaxBins bins (one pass where shared memory holds k + 1 bins,
 // else 2 or 3 by digits, least significant first); a slot is ranked among its warp's equal
 // keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit counters per warp
-// and bin.  Up to kClusterSlots slots one cluster of at most 8 blocks runs all passes: the
-// blocks' totals are exchanged through distributed shared memory, so a pass costs two
-// cluster barriers and no launch.  More slots take three kernels a pass (histograms of
-// tiles, scan of each bin over the tiles, scatter through shared memory so that a bin's run
-// is stored together).  The sort moves 4 to 8 bytes a slot where the rows move kilobytes;
-// the row kernels are bound by HBM, and read and write every row once: a row's copies are
-// written from registers after one read, its weighted sum is formed from p reads.
-#include "common.cuh"
+// and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in 2.7 us.  More take
+// three kernels a pass (histograms of tiles, scan of each bin over the tiles, scatter through
+// shared memory so that a bin's run is stored together), 131072 slots of 128 labels in 8.3
+// us, 8192 of 256 in 8.5 (one block 23); one cluster of 8 blocks took 54 for them, since eight SMs scatter no faster.  The sort
+// moves 4 to 8 bytes a slot where the rows move kilobytes; the row kernels are bound by HBM,
+// and read and write every row once: a row's copies are written from registers after one
+// read, its weighted sum is formed from p reads.
 #include "engine.h"
 #include "rows.cuh"
 
@@ -29,8 +28,9 @@
 namespace euc {
 
 // ------------------------------------------------------------------ the sort
-constexpr int kMaxBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass
-constexpr int kPassBits = 11;   // digits of a sort of several passes, at most
+constexpr int kBlockBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass of a block,
+constexpr int kMaxBins = 4609;    // and of three kernels: what shared memory holds per warp and bin
+constexpr int kPassBits = 11;     // digits of a sort of several passes, at most
 
 struct SortOut {
   uint32_t* keys;  // a pass that is not the last: keys and slots in the pass's order
@@ -88,29 +88,27 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], unsig
   }
 }
 
-// ---- all passes in one cluster
-struct ClusterSort {
-  int64_t n;
+// ---- all passes in one block
+struct BlockSort {
+  int n;
   uint32_t k;
-  int passes, bits, bins, log_cluster;
+  int passes, bits, bins;
   uint32_t *keys[2], *slots[2];  // between passes
 };
 
-constexpr int kClusterItems = 2;
-constexpr int64_t kClusterSlots = 8 * 1024 * kClusterItems;  // more scatter faster from every SM than from eight
+constexpr int kBlockItems = 2;
+constexpr int64_t kBlockSlots = 1024 * kBlockItems;
 
 template <typename TL, int ITEMS>
-__global__ void __launch_bounds__(1024) sort_cluster_kernel(const TL* __restrict__ in, ClusterSort a, SortOut o) {
+__global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__ in, BlockSort a, SortOut o) {
   extern __shared__ uint32_t sm[];
   __shared__ uint32_t warp_sums[32];
+  let_next_start();
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cluster = 1 << a.log_cluster, rank_in = static_cast<int>(blockIdx.x);
-  uint32_t* total = sm;               // [bins] this block's slots per digit
-  uint32_t* start = sm + a.bins;      // [bins] first position of this block's slots
-  uint32_t* before = sm + 2 * a.bins;  // [bins] slots of the cluster's earlier blocks per digit
-  unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + 3 * a.bins);  // [warps][bins]
+  uint32_t* start = sm;  // [bins] first position of the digit
+  unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + a.bins);  // [warps][bins]
   unsigned short* mine = cnt + warp * a.bins;
-  const int64_t base = (static_cast<int64_t>(rank_in) * warps + warp) * (32 * ITEMS) + lane;
+  const int base = warp * (32 * ITEMS) + lane;
   for (int pass = 0; pass < a.passes; ++pass) {
     const bool last = pass == a.passes - 1;
     const int shift = pass * a.bits;
@@ -121,7 +119,7 @@ __global__ void __launch_bounds__(1024) sort_cluster_kernel(const TL* __restrict
     unsigned short rank[ITEMS];
 #pragma unroll
     for (int u = 0; u < ITEMS; ++u) {
-      const int64_t s = base + u * 32;
+      const int s = base + u * 32;
       key[u] = s >= a.n ? 0u : pass == 0 ? key_of(in[s], a.k) : __ldcg(from_keys + s);
       digit[u] = s >= a.n ? 0xffffffffu : (key[u] >> shift) & mask;
     }
@@ -136,33 +134,17 @@ __global__ void __launch_bounds__(1024) sort_cluster_kernel(const TL* __restrict
         cnt[w * a.bins + c] = static_cast<unsigned short>(run);
         run += t;
       }
-      total[c] = run;
       start[c] = run;
     }
     __syncthreads();
-    if (cluster > 1) {
-      cluster_sync();
-      for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {
-        uint32_t all = 0u, earlier = 0u;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const uint32_t t = r < cluster ? load_cluster_u32(total + c, static_cast<uint32_t>(r)) : 0u;
-          all += t;
-          earlier += r < rank_in ? t : 0u;
-        }
-        start[c] = all;
-        before[c] = earlier;
-      }
-      __syncthreads();
-    }
     block_scan(start, a.bins, warp_sums);
-    if (last && o.offsets && rank_in == 0)
+    if (last && o.offsets)
       for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
 #pragma unroll
     for (int u = 0; u < ITEMS; ++u) {
-      const int64_t s = base + u * 32;
+      const int s = base + u * 32;
       if (s >= a.n) continue;
-      const uint32_t pos = start[digit[u]] + (cluster > 1 ? before[digit[u]] : 0u) + mine[digit[u]] + rank[u];
+      const uint32_t pos = start[digit[u]] + mine[digit[u]] + rank[u];
       const uint32_t slot = pass == 0 ? static_cast<uint32_t>(s) : __ldcg(from_slots + s);
       if (last) {
         const bool kept = key[u] < a.k;
@@ -174,15 +156,13 @@ __global__ void __launch_bounds__(1024) sort_cluster_kernel(const TL* __restrict
         a.slots[pass & 1][pos] = slot;
       }
     }
-    // the next pass reads what every block wrote, and none leaves while its totals are read
-    __syncthreads();
-    if (cluster > 1) cluster_sync();
+    __syncthreads();  // the next pass reads what this one wrote
   }
 }
 
 // ---- three kernels a pass
-constexpr int kTileWarps = 8;
-constexpr int kTileItems = 8;
+constexpr int kTileWarps = 16;
+constexpr int kTileItems = 4;
 constexpr int kTile = kTileWarps * 32 * kTileItems;  // 2048 slots, so 16 bits index one of them
 
 struct SortPass {
@@ -204,7 +184,9 @@ template <typename TL, bool FIRST> __device__ __forceinline__ uint32_t load_key(
 template <typename TL, bool FIRST>
 __global__ void __launch_bounds__(kTileWarps * 32) sort_hist_kernel(const TL* __restrict__ in, SortPass a) {
   extern __shared__ uint32_t cnt[];
+  let_next_start();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) cnt[c] = 0u;
+  if (!FIRST) wait_for_previous();
   __syncthreads();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x;
   uint32_t key[kTileItems];
@@ -228,6 +210,8 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_hist_kernel(const TL* __
 // one warp per bin: T[bin][.] becomes its exclusive prefix over the tiles, 512 tiles at a time
 __global__ void __launch_bounds__(256) sort_tiles_kernel(SortPass a) {
   const int bin = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  let_next_start();
+  wait_for_previous();
   if (bin >= a.bins) return;
   uint4* row = reinterpret_cast<uint4*>(a.T + static_cast<int64_t>(bin) * a.tiles);
   const int quads = a.tiles / 4;
@@ -273,12 +257,15 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
   uint32_t* local = sm + a.bins;         // [bins] less its position in the tile
   uint32_t* stage = sm + 2 * a.bins;     // [kTile] digit and slot, in the tile's order
   unsigned short* cnt = reinterpret_cast<unsigned short*>(stage + kTile);  // [warps][bins]
-  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) start[c] = a.total[c];
-  for (int c = threadIdx.x; c < a.bins * kTileWarps; c += blockDim.x) cnt[c] = 0;
+  let_next_start();
+  for (int c = threadIdx.x; c < a.bins * (kTileWarps / 2); c += blockDim.x) reinterpret_cast<uint32_t*>(cnt)[c] = 0u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned short* mine = cnt + warp * a.bins;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * kTile;
   const int first = warp * (32 * kTileItems) + lane;
+  // the ranks within the tile need the labels alone (of a first pass: what came before the
+  // sort), so they are formed while the histograms are still being summed
+  if (!FIRST) wait_for_previous();
   uint32_t digit[kTileItems];
   unsigned short rank[kTileItems];
 #pragma unroll
@@ -287,9 +274,6 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
     digit[u] = s < a.n ? (load_key<TL, FIRST>(in, s, a.k) >> a.shift) & a.mask : 0xffffffffu;
   }
   __syncthreads();
-  block_scan(start, a.bins, warp_sums);
-  if (LAST && o.offsets && blockIdx.x == 0)
-    for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
   warp_ranks<kTileItems>(digit, rank, mine, lane);
   __syncthreads();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
@@ -304,26 +288,36 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
   }
   __syncthreads();
   block_scan(local, a.bins, warp_sums);
+  if (FIRST) wait_for_previous();
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) start[c] = a.total[c];
+  __syncthreads();
+  block_scan(start, a.bins, warp_sums);
+  if (LAST && o.offsets && blockIdx.x == 0)
+    for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x)  // (every thread its own bins, as above)
+    start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] - local[c];
+  __syncthreads();
 #pragma unroll
   for (int u = 0; u < kTileItems; ++u)
-    if (digit[u] != 0xffffffffu)
-      stage[local[digit[u]] + mine[digit[u]] + rank[u]] = (digit[u] << 16) | static_cast<uint32_t>(first + u * 32);
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.bins; c += blockDim.x)
-    start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] - local[c];
+    if (digit[u] != 0xffffffffu) {
+      const uint32_t l = local[digit[u]] + mine[digit[u]] + rank[u];
+      stage[l] = (digit[u] << 16) | static_cast<uint32_t>(first + u * 32);
+      // of a sort of one pass the digit is the key, and neighbouring lanes have neighbouring slots
+      if (FIRST && LAST) o.position[tile + first + u * 32] = digit[u] < a.k ? static_cast<int32_t>(start[digit[u]] + l) : -1;
+    }
   __syncthreads();
   const int here = static_cast<int>(min(static_cast<int64_t>(kTile), a.n - tile));
   for (int l = threadIdx.x; l < here; l += blockDim.x) {
     const uint32_t w = stage[l], d = w >> 16;
     const int64_t s = tile + (w & 0xffffu);
     const uint32_t pos = start[d] + l;
-    const uint32_t key = load_key<TL, FIRST>(in, s, a.k);
+    const uint32_t key = FIRST && LAST ? d : load_key<TL, FIRST>(in, s, a.k);
     const uint32_t slot = FIRST ? static_cast<uint32_t>(s) : in_slots[s];
     if (LAST) {
       const bool kept = key < a.k;
       o.order[pos] = kept ? static_cast<int32_t>(slot) : -1;
       o.labels[pos] = kept ? static_cast<int32_t>(key) : -1;
-      o.position[slot] = kept ? static_cast<int32_t>(pos) : -1;
+      if (!FIRST) o.position[slot] = kept ? static_cast<int32_t>(pos) : -1;
     } else {
       o.keys[pos] = key;
       o.slots[pos] = slot;
@@ -334,6 +328,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
 // offsets of a sort of several passes: first position whose key is not below c
 __global__ void sort_offsets_kernel(const int32_t* __restrict__ labels, int64_t n, int64_t k,
                                     int32_t* __restrict__ offsets) {
+  wait_for_previous();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (c > k) return;
   int64_t lo = 0, hi = n;  // dropped slots (-1, at the end) count as k
@@ -349,14 +344,14 @@ static inline size_t al(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct SortPlan {
   int passes, bits, bins, tiles;
-  bool cluster;
+  bool block;
 };
 
 static SortPlan sort_plan(int64_t n, int64_t k) {
   SortPlan p{};
-  p.cluster = n <= kClusterSlots;
+  p.block = n <= kBlockSlots;
   p.tiles = static_cast<int>(((n + kTile - 1) / kTile + 3) / 4 * 4);
-  if (k + 1 <= kMaxBins) {
+  if (k + 1 <= (p.block ? kBlockBins : kMaxBins)) {
     p.passes = 1;
     p.bins = static_cast<int>(k + 1);
     return p;
@@ -373,55 +368,52 @@ size_t group_ws_bytes(int64_t n, int64_t k) {
   if (n <= 0) return 0;
   const SortPlan p = sort_plan(n, k);
   size_t b = 0;
-  if (!p.cluster) b += al(static_cast<size_t>(p.bins) * p.tiles * 4) + al(static_cast<size_t>(p.bins) * 4);
+  if (!p.block) b += al(static_cast<size_t>(p.bins) * p.tiles * 4) + al(static_cast<size_t>(p.bins) * 4);
   if (p.passes > 1) b += 2 * al(static_cast<size_t>(n) * 4);
   if (p.passes > 2) b += 2 * al(static_cast<size_t>(n) * 4);
   return b;
 }
 
+// dynamic shared memory beyond the 48 KiB that a launch may ask for unannounced, of which the
+// kernels' static arrays take a little
 static cudaError_t more_smem(const void* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return cudaSuccess;
+  if (bytes <= 47 * 1024) return cudaSuccess;
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
 template <typename TL, int ITEMS>
-static cudaError_t sort_cluster(const TL* in, ClusterSort a, const SortOut& o, cudaStream_t st) {
-  // blocks of 1024 threads, as many as hold the slots; one block no larger than the slots
-  int64_t threads = (a.n + ITEMS - 1) / ITEMS;
-  int cluster = 1;
-  while (static_cast<int64_t>(cluster) * 1024 < threads) {
-    cluster *= 2;
-    ++a.log_cluster;
-  }
-  const int nt = cluster > 1 ? 1024 : static_cast<int>((threads + 31) / 32 * 32);
-  const size_t smem = static_cast<size_t>(a.bins) * (12 + 2 * (nt / 32));
-  cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_cluster_kernel<TL, ITEMS>), smem);
+static cudaError_t sort_block(const TL* in, const BlockSort& a, const SortOut& o, cudaStream_t st) {
+  const int nt = ((a.n + ITEMS - 1) / ITEMS + 31) / 32 * 32;
+  const size_t smem = static_cast<size_t>(a.bins) * (4 + 2 * (nt / 32));
+  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_block_kernel<TL, ITEMS>), smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(cluster));
-  cfg.blockDim = dim3(static_cast<unsigned>(nt));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, sort_cluster_kernel<TL, ITEMS>, in, a, o);
+  sort_block_kernel<TL, ITEMS><<<1, nt, smem, st>>>(in, a, o);
+  return cudaGetLastError();
 }
 
 template <typename TL, bool FIRST, bool LAST>
 static cudaError_t sort_pass(const TL* in, const uint32_t* in_slots, const SortPass& a, const SortOut& o,
                              cudaStream_t st) {
   const size_t sm = static_cast<size_t>(a.bins) * (8 + 2 * kTileWarps) + kTile * 4;
-  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_scatter_kernel<TL, FIRST, LAST>), sm);
+  cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_scatter_kernel<TL, FIRST, LAST>), sm);
   if (e != cudaSuccess) return e;
   const unsigned tiles = static_cast<unsigned>((a.n + kTile - 1) / kTile);
-  sort_hist_kernel<TL, FIRST><<<tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st>>>(in, a);
-  sort_tiles_kernel<<<(a.bins + 7) / 8, 256, 0, st>>>(a);
-  sort_scatter_kernel<TL, FIRST, LAST><<<tiles, kTileWarps * 32, sm, st>>>(in, in_slots, a, o);
-  return cudaGetLastError();
+  // Each kernel may start while the one before it runs, if all their blocks fit beside one
+  // another with little shared memory: 131072 slots of 128 labels take 8.1 us so, and 11.4
+  // one after another; but 1048576 slots of 1024 labels 40 us, and 33 one after another.
+  const bool early = a.bins <= 512 && static_cast<int>(tiles) <= num_sms();
+  if (FIRST || !early) {
+    sort_hist_kernel<TL, FIRST><<<tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st>>>(in, a);
+    e = cudaGetLastError();
+  } else {
+    e = launch_after(true, sort_hist_kernel<TL, FIRST>, tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st, in,
+                     a);
+  }
+  if (e == cudaSuccess)
+    e = launch_after(early, sort_tiles_kernel, static_cast<unsigned>((a.bins + 7) / 8), 256, 0, st, a);
+  if (e == cudaSuccess)
+    e = launch_after(early, sort_scatter_kernel<TL, FIRST, LAST>, tiles, kTileWarps * 32, sm, st, in, in_slots, a, o);
+  return e;
 }
 
 template <typename TL>
@@ -439,9 +431,9 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
     ws += al(static_cast<size_t>(n) * 4);
   }
   cudaError_t e = cudaSuccess;
-  if (p.cluster) {
-    ClusterSort a{};
-    a.n = n;
+  if (p.block) {
+    BlockSort a{};
+    a.n = static_cast<int>(n);
     a.k = static_cast<uint32_t>(k);
     a.passes = p.passes;
     a.bits = p.bits;
@@ -450,7 +442,7 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
       a.keys[i] = buf[2 * i];
       a.slots[i] = buf[2 * i + 1];
     }
-    e = n <= 8 * 1024 ? sort_cluster<TL, 1>(labels, a, o, st) : sort_cluster<TL, kClusterItems>(labels, a, o, st);
+    e = n <= 1024 ? sort_block<TL, 1>(labels, a, o, st) : sort_block<TL, kBlockItems>(labels, a, o, st);
   } else {
     SortPass a{};
     a.n = n;
@@ -479,10 +471,8 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
     a.shift = p.bits * (p.passes - 1);
     if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(keys, slots, a, o, st);
   }
-  if (e == cudaSuccess && p.passes > 1) {
-    sort_offsets_kernel<<<static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st>>>(sorted, n, k, offsets);
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess && p.passes > 1)
+    e = launch_after(true, sort_offsets_kernel, static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st, sorted, n, k, offsets);
   return e;
 }
 
@@ -583,24 +573,26 @@ __global__ void __launch_bounds__(256) rows_from_groups_kernel(const T* __restri
   for (int j0 = 0; j0 < p; j0 += J) {
     V z[J][U];
     A wt[J];
+    bool ok[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int64_t r = j0 + j < p ? pos[j0 + j] : -1;
-      const bool ok = r >= 0 && r < slots;
+      ok[j] = r >= 0 && r < slots;
       wt[j] = WEIGHTED && j0 + j < p ? wts[j0 + j] : A(1);
-      wt[j] = ok ? wt[j] : A(0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         z[j][u].raw = raw_zero<Raw>();
-        if (ok && v + 32 * u < nv) z[j][u].raw = load_once(Zr + r * nv + v + 32 * u);
+        if (ok[j] && v + 32 * u < nv) z[j][u].raw = load_once(Zr + r * nv + v + 32 * u);
       }
     }
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < J; ++j) {  // (the weight is first looked at here, behind the rows' loads)
+      const A w = ok[j] ? wt[j] : A(0);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[u][e] += wt[j] * to_acc(z[j][u].e[e]);
+        for (int e = 0; e < N; ++e) acc[u][e] += w * to_acc(z[j][u].e[e]);
+    }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -613,10 +605,17 @@ __global__ void __launch_bounds__(256) rows_from_groups_kernel(const T* __restri
 }
 
 // ------------------------------------------------------------------ the way back's gradient
-// A team of 32 TEAM_WARPS threads per row: dOut[i] stays in L1 while the row's picks are
-// walked; each thread keeps the partial products of up to 4 picks, summed over the team in
-// a fixed order.
-template <typename T, int N, int TEAM_WARPS>
+// A team of 8, 32 or 256 threads per row, J picks at a time: dOut[i] is read once for all of
+// them (and again, from L1, for the next J), each thread keeps its partial products of the J
+// picks, and they are summed over the team in a fixed order.
+template <int TEAM, typename A, int J> __device__ __forceinline__ void team_dots(A (&dot)[J], int lane) {
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int s = (TEAM < 32 ? TEAM : 32) / 2; s > 0; s >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], s);
+}
+
+template <typename T, int N, int TEAM, int J>
 __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
     const T* __restrict__ G, const T* __restrict__ Z, const int32_t* __restrict__ position,
     const Acc<T>* __restrict__ weights, const int32_t* __restrict__ kept, int64_t n, int p, int64_t nv,
@@ -624,86 +623,79 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
   using A = Acc<T>;
   using V = Vec<T, N>;
   using Raw = typename V::Raw;
-  constexpr int TEAMS = 8 / TEAM_WARPS;
-  constexpr int UV = N * sizeof(T) >= 16 ? 1 : N * sizeof(T) == 8 ? 2 : 4;  // vectors in flight, with each pick's
-  __shared__ A part[8][4];
+  constexpr int TEAMS = 256 / TEAM;
+  constexpr int BYTES = N * static_cast<int>(sizeof(T));
+  constexpr int UV = BYTES >= 16 ? (J > 2 ? 1 : 2) : BYTES == 8 ? 2 : 4;  // vectors in flight, with each pick's
+  __shared__ A part[8][J];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int team = warp / TEAM_WARPS, in_team = threadIdx.x - team * TEAM_WARPS * 32;
+  const int team = static_cast<int>(threadIdx.x) / TEAM, in_team = static_cast<int>(threadIdx.x) % TEAM;
   const int64_t slots = n * p;
   const Raw* Gr = reinterpret_cast<const Raw*>(G);
   const Raw* Zr = reinterpret_cast<const Raw*>(Z);
   Raw* gZr = reinterpret_cast<Raw*>(gZ);
-  // every team of a block takes the same number of turns, for the block barriers below
+  // every team of a block takes the same number of turns, for the barriers below
   for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * TEAMS; i0 < n; i0 += static_cast<int64_t>(gridDim.x) * TEAMS) {
     const int64_t i = i0 + team;
-    for (int j0 = 0; j0 < p; j0 += 4) {
-      A dot[4] = {A(0), A(0), A(0), A(0)};
-      if (i < n) {
-        int64_t r[4];
-        A wt[4];
+    for (int j0 = 0; j0 < p; j0 += J) {
+      A dot[J];
+      int64_t r[J];
+      A wt[J];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          r[u] = j0 + u < p ? position[i * p + j0 + u] : -1;
-          if (r[u] >= slots) r[u] = -1;
-          wt[u] = r[u] >= 0 ? (weights ? weights[i * p + j0 + u] : A(1)) : A(0);
+      for (int j = 0; j < J; ++j) {
+        dot[j] = A(0);
+        r[j] = i < n && j0 + j < p ? position[i * p + j0 + j] : -1;
+        if (r[j] >= slots) r[j] = -1;
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) wt[j] = weights && i < n && j0 + j < p ? weights[i * p + j0 + j] : A(1);
+      for (int64_t v0 = in_team; v0 < nv && i < n; v0 += UV * TEAM) {
+        V g[UV], z[UV][J];
+#pragma unroll
+        for (int q = 0; q < UV; ++q) {
+          const int64_t v = v0 + q * TEAM;
+          g[q].raw = raw_zero<Raw>();
+          if (v < nv) g[q].raw = load_keep(Gr + i * nv + v);
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            z[q][j].raw = raw_zero<Raw>();
+            if (gW && r[j] >= 0 && v < nv) z[q][j].raw = load_once(Zr + r[j] * nv + v);
+          }
         }
-        for (int64_t v0 = in_team; v0 < nv; v0 += UV * TEAM_WARPS * 32) {
-          V g[UV], z[UV][4];
 #pragma unroll
-          for (int q = 0; q < UV; ++q) {
-            const int64_t v = v0 + q * (TEAM_WARPS * 32);
-            g[q].raw = raw_zero<Raw>();
-            if (v < nv) g[q].raw = load_keep(Gr + i * nv + v);
-            if (gW) {
+        for (int q = 0; q < UV; ++q) {
+          const int64_t v = v0 + q * TEAM;
+          if (v >= nv) continue;
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                z[q][u].raw = raw_zero<Raw>();
-                if (r[u] >= 0 && v < nv) z[q][u].raw = load_once(Zr + r[u] * nv + v);
-              }
-            }
-          }
+          for (int j = 0; j < J; ++j)
+            if (gW && r[j] >= 0) {
 #pragma unroll
-          for (int q = 0; q < UV; ++q) {
-            const int64_t v = v0 + q * (TEAM_WARPS * 32);
-            if (v >= nv) continue;
-            if (gW) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                if (r[u] >= 0) {
-#pragma unroll
-                  for (int e = 0; e < N; ++e) dot[u] += to_acc(g[q].e[e]) * to_acc(z[q][u].e[e]);
-                }
+              for (int e = 0; e < N; ++e) dot[j] += to_acc(g[q].e[e]) * to_acc(z[q][j].e[e]);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (r[u] >= 0) {
-                V o;
+          for (int j = 0; j < J; ++j)
+            if (r[j] >= 0) {
+              V o;
 #pragma unroll
-                for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(wt[u] * to_acc(g[q].e[e]));
-                store_once(gZr + r[u] * nv + v, o.raw);
-              }
-          }
+              for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(wt[j] * to_acc(g[q].e[e]));
+              store_once(gZr + r[j] * nv + v, o.raw);
+            }
         }
       }
       if (gW) {
+        team_dots<TEAM>(dot, lane);
+        if (TEAM <= 32) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int s = 16; s > 0; s >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], s);
-        if (TEAM_WARPS == 1) {
-          if (lane == 0 && i < n)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (j0 + u < p) gW[i * p + j0 + u] = dot[u];
+          for (int j = 0; j < J; ++j)
+            if (in_team == j % TEAM && i < n && j0 + j < p) gW[i * p + j0 + j] = dot[j];
         } else {
           if (lane == 0)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) part[warp][u] = dot[u];
+            for (int j = 0; j < J; ++j) part[warp][j] = dot[j];
           __syncthreads();
-          if (in_team < 4 && i < n && j0 + in_team < p) {
+          if (in_team < J && i < n && j0 + in_team < p) {
             A s = A(0);
 #pragma unroll
-            for (int q = 0; q < TEAM_WARPS; ++q) s += part[team * TEAM_WARPS + q][in_team];
+            for (int w = 0; w < 8; ++w) s += part[w][in_team];
             gW[i * p + j0 + in_team] = s;
           }
           __syncthreads();
@@ -761,7 +753,7 @@ cudaError_t launch_rows_to_groups(int esize, const void* X, const int32_t* posit
 template <typename T, int N, int J, bool WEIGHTED>
 static cudaError_t from_groups_j(const T* Z, const int32_t* position, const Acc<T>* w, int64_t n, int p, int64_t nv,
                                  T* out, cudaStream_t st) {
-  constexpr int U = N * sizeof(T) >= 8 ? 1 : 4;
+  constexpr int U = N * sizeof(T) >= 8 ? 2 : 4;
   if (nv >= 32)
     rows_from_groups_kernel<T, N, J, U, WEIGHTED, true><<<static_cast<unsigned>(wide_blocks(n, nv, 1, U)), 256, 0, st>>>(
         Z, position, w, n, p, nv, (nv + 32 * U - 1) / (32 * U), out);
@@ -787,22 +779,33 @@ static cudaError_t from_groups_n(const T* Z, const int32_t* position, const void
            : from_groups_w<T, N, false>(Z, position, w, n, p, dim / N, out, st);
 }
 
+template <typename T, int N, int TEAM>
+static cudaError_t from_groups_grad_team(const T* G, const T* Z, const int32_t* position, const void* weights,
+                                         const int32_t* kept, int64_t n, int p, int64_t nv, T* gZ, void* gW,
+                                         cudaStream_t st) {
+  const Acc<T>* w = static_cast<const Acc<T>*>(weights);
+  Acc<T>* gw = static_cast<Acc<T>*>(gW);
+  const unsigned g = static_cast<unsigned>(
+      std::min<int64_t>((n * TEAM + 255) / 256, static_cast<int64_t>(num_sms()) * 64));
+  if (p == 1)
+    rows_from_groups_grad_kernel<T, N, TEAM, 1><<<g, 256, 0, st>>>(G, Z, position, w, kept, n, p, nv, gZ, gw);
+  else if (p == 2)
+    rows_from_groups_grad_kernel<T, N, TEAM, 2><<<g, 256, 0, st>>>(G, Z, position, w, kept, n, p, nv, gZ, gw);
+  else
+    rows_from_groups_grad_kernel<T, N, TEAM, 4><<<g, 256, 0, st>>>(G, Z, position, w, kept, n, p, nv, gZ, gw);
+  return cudaGetLastError();
+}
+
 template <typename T, int N>
 static cudaError_t from_groups_grad_n(const T* G, const T* Z, const int32_t* position, const void* weights,
                                       const int32_t* kept, int64_t n, int p, int64_t dim, T* gZ, void* gW,
                                       cudaStream_t st) {
   const int64_t nv = dim / N;
-  const Acc<T>* w = static_cast<const Acc<T>*>(weights);
-  Acc<T>* gw = static_cast<Acc<T>*>(gW);
-  const int64_t most = static_cast<int64_t>(num_sms()) * 64;
-  // a block per row, for what it has in flight; a warp where the row is no longer than that
-  if (nv <= 64)
-    rows_from_groups_grad_kernel<T, N, 1><<<static_cast<unsigned>(std::min<int64_t>((n + 7) / 8, most)), 256, 0, st>>>(
-        G, Z, position, w, kept, n, p, nv, gZ, gw);
-  else
-    rows_from_groups_grad_kernel<T, N, 8><<<static_cast<unsigned>(std::min<int64_t>(n, most)), 256, 0, st>>>(
-        G, Z, position, w, kept, n, p, nv, gZ, gw);
-  return cudaGetLastError();
+  // as many threads per row as it has vectors to give them; blocks of 256 where there are few rows
+  if (nv <= 16) return from_groups_grad_team<T, N, 8>(G, Z, position, weights, kept, n, p, nv, gZ, gW, st);
+  if (nv <= 64 || (nv <= 384 && n >= static_cast<int64_t>(num_sms()) * 32))
+    return from_groups_grad_team<T, N, 32>(G, Z, position, weights, kept, n, p, nv, gZ, gW, st);
+  return from_groups_grad_team<T, N, 256>(G, Z, position, weights, kept, n, p, nv, gZ, gW, st);
 }
 
 template <typename T>

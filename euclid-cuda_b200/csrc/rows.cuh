@@ -62,6 +62,28 @@ inline int row_vec_bytes(int64_t row_bytes, uintptr_t addresses) {
   return (a & 15u) == 0 ? 16 : (a & 7u) == 0 ? 8 : (a & 3u) == 0 ? 4 : 2;
 }
 
+// Programmatic dependent launch: a kernel launched with `early` may start while the one before
+// it on the stream still runs; what it does before wait_for_previous() reads nothing
+// that kernel writes and writes nothing that it touches.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... Q>
+inline cudaError_t launch_after(bool early, void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+                                Q... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // How the row kernels cut rows of nv vectors into work (kUnit threads' worth a block).
 //
 // Wide rows (nv >= 32): a warp takes R neighbouring rows times a chunk of 32 U vectors, so a

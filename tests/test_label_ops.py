@@ -91,7 +91,7 @@ def test_groups_abi_checks(lib):
     big = 2 ** 31 - 1
     assert lib.euc_group_rows_workspace_bytes(0, 5) == 0
     assert lib.euc_group_rows_workspace_bytes(big, 5) == 0 and lib.euc_group_rows_workspace_bytes(5, big) == 0
-    # one cluster, one pass: none; several passes keep keys and slots between them; many slots
+    # one block, one pass: none; several passes keep keys and slots between them; many slots
     # keep a histogram per tile too
     assert lib.euc_group_rows_workspace_bytes(1000, 64) == 0
     assert lib.euc_group_rows_workspace_bytes(1000, 100000) >= 2 * 4000
