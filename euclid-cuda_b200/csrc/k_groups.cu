@@ -29,7 +29,7 @@ namespace euc {
 
 // ------------------------------------------------------------------ the sort
 constexpr int kBlockBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass of a block,
-constexpr int kMaxBins = 4609;    // and of three kernels: what shared memory holds per warp and bin
+constexpr int kMaxBins = 1537;    // and of three kernels (1048576 slots of 4000 labels: 50 us in two passes, 94 in one)
 constexpr int kPassBits = 11;     // digits of a sort of several passes, at most
 
 struct SortOut {

@@ -238,6 +238,13 @@ template <typename T> struct RowVecs {
     flip_even = sizeof(T) == 8 ? 0u : flip_odd;
   }
   __device__ __forceinline__ uint4 read(int v) const { return load_keep(base + v); }
+  // 16 bytes of masked scores
+  __device__ __forceinline__ uint4 masked() const {
+    Vec<T, VE> v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v.e[e] = from_acc<T>(flip_odd ? -neg_inf<Acc<T>>() : neg_inf<Acc<T>>());
+    return v.raw;
+  }
   __device__ __forceinline__ void values(uint4 w, Acc<T>* y) const {
     w.x ^= flip_even;
     w.y ^= flip_odd;
@@ -374,61 +381,76 @@ template <typename A> __device__ __forceinline__ int place_of(const Key<A>* list
 // ------------------------------------------------------------------ a team of lanes per row
 // Rows of up to TEAM EPL scores, a team of 8 or 32 lanes each: the row stays in registers, so
 // its scores are read once and its maximum is known before the first exponential; a warp
-// reads its next rows while it works on these (not with 64 scores a lane, whose registers
-// are better spent on more warps).  FLAT: every row is whole 16-byte vectors;
+// reads its next rows while it works on these, into shared memory, which leaves the registers
+// to more warps.  FLAT: every row is whole 16-byte vectors;
 // other rows are read element by element, neighbouring lanes neighbouring elements.
-constexpr int kTeamCands = 256;  // per warp
+template <int TEAM> constexpr int kTeamCands = TEAM == 8 ? 64 : TEAM == 16 ? 96 : 128;
+
+__device__ __forceinline__ void copy_async_16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <typename T, int TEAM, int EPL, bool FLAT>
-__global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) >= 256 ? (sizeof(T) == 8 ? 2 : 4) : 5) scores_team_kernel(ScoreArgs<T> a) {
+__global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) == 8 ? 2 : 4) : (FLAT ? 7 : 5))
+    scores_team_kernel(ScoreArgs<T> a) {
   using A = Acc<T>;
-  constexpr int VE = FLAT ? RowVecs<T>::VE : 1, NV = EPL / VE, RPW = 32 / TEAM, CAP = kTeamCands / RPW;
-  constexpr bool AHEAD = EPL <= 32;
-  __shared__ Key<A> cands[4][kTeamCands];
+  constexpr int VE = FLAT ? RowVecs<T>::VE : 1, NV = EPL / VE, RPW = 32 / TEAM, CAP = kTeamCands<TEAM>;
+  // FLAT: where a lane's vectors of the next row land; each lane reads its own alone
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ Key<A> cands[4][CAP * RPW];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tl = lane % TEAM, team = lane / TEAM;
   const unsigned team_lanes = (TEAM == 32 ? 0xffffffffu : (1u << (TEAM & 31)) - 1u) << (team * TEAM);
   const unsigned before_me = team_lanes & ((1u << lane) - 1u);
   const bool negate = a.sign < A(0);
   const A c = a.mag * Expo<A>::per_nat;
   Key<A>* list = cands[warp] + team * CAP;
+  uint4* slot = reinterpret_cast<uint4*>(dyn) + (warp * NV) * 32 + lane;  // (v-th vector: slot[v * 32])
   const int64_t step = static_cast<int64_t>(gridDim.x) * (4 * RPW);
   int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + warp) * RPW;
   if (first >= a.n) return;
-  using Raw = typename std::conditional<FLAT, uint4, T>::type;
-  Raw next[NV];
+  T next[FLAT ? 1 : EPL];
   int64_t next_label = -1;
-  // vectors behind the row's end hold z = -inf from the start, and no load changes them
+  // elements behind the row's end hold z = -inf from the start, and no load changes them
+  const RowVecs<T> any(a.x, a.m, negate);
+  if constexpr (FLAT) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    Vec<T, FLAT ? VE : 1> fill;
+    for (int v = 0; v < NV; ++v) slot[v * 32] = any.masked();
+  } else {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) fill.e[e] = from_acc<T>(negate ? -neg_inf<A>() : neg_inf<A>());
-    if constexpr (FLAT) next[v] = fill.raw;
-    else next[v] = fill.e[0];
+    for (int v = 0; v < NV; ++v) next[v] = from_acc<T>(negate ? -neg_inf<A>() : neg_inf<A>());
   }
   auto fetch = [&](int64_t row) {
     row = min(row, a.n - 1);
     const T* x = a.x + row * a.ld;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if ((v * TEAM + tl) * VE < a.m) next[v] = load_keep(reinterpret_cast<const Raw*>(x) + v * TEAM + tl);
+      if ((v * TEAM + tl) * VE < a.m) {
+        if constexpr (FLAT) copy_async_16(slot + v * 32, reinterpret_cast<const uint4*>(x) + v * TEAM + tl);
+        else next[v] = load_keep(x + v * TEAM + tl);
+      }
     if (a.log_probs) next_label = label_of<T>(a.labels, a.labels_i64, row);
   };
-  if (AHEAD) fetch(first + team);
+  fetch(first + team);
   for (; first < a.n; first += step) {
-    if (!AHEAD) fetch(first + team);
-    const bool live = first + team < a.n;
+    const bool live = first + team < a.n, more = first + step < a.n;
     const int64_t i = live ? first + team : a.n - 1;
     const RowVecs<T> row(a.x + i * a.ld, a.m, negate);
     A y[EPL];
+    if constexpr (FLAT) {
+      copy_async_wait();
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      if constexpr (FLAT) row.values(next[v], y + v * VE);
-      else y[v] = negate ? -to_acc(next[v]) : to_acc(next[v]);
+      for (int v = 0; v < NV; ++v) row.values(slot[v * 32], y + v * VE);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) y[v] = negate ? -to_acc(next[v]) : to_acc(next[v]);
     }
     const bool labelled = next_label >= 0 && next_label < a.m;
     const A at_label = labelled ? row.at(static_cast<int>(next_label)) : A(0);  // ready by the time it is needed
-    if (AHEAD && first + step < a.n) fetch(first + step + team);
+    // the next row is on its way while this one is worked on; with alternatives, a row in
+    // shared memory stays until its candidates are read from there
+    const bool early = !FLAT || a.top == 0;
+    if (early && more) fetch(first + step + team);
     A lists[4];
 #pragma unroll
     for (int l = 0; l < 4; ++l) lists[l] = max_of<A, EPL / 4>(y + l * (EPL / 4));
@@ -459,21 +481,32 @@ __global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) >= 256 ? (sizeof(T) 
     }
 #pragma unroll
     for (int w = 0; w < EPL; w += 32) {
-      uint32_t in = 0u;
+      uint32_t part[4] = {0u, 0u, 0u, 0u};  // (four chains of dependent instructions instead of one)
 #pragma unroll
-      for (int q = 0; q < (EPL < 32 ? EPL : 32); ++q) in |= y[w + q] >= t ? 1u << q : 0u;
+      for (int q = 0; q < (EPL < 32 ? EPL : 32); ++q) part[q % 4] |= y[w + q] >= t ? 1u << q : 0u;
+      uint32_t in = (part[0] | part[1]) | (part[2] | part[3]);
       while (true) {
         const unsigned b = __ballot_sync(0xffffffffu, in != 0u);
         if (b == 0u) break;
         if (in != 0u) {
           const int at = count + __popc(b & before_me), q = w + __ffs(in) - 1;
           const int j = ((q / VE) * TEAM + tl) * VE + q % VE;
-          if (at < CAP) list[at] = Key<A>::of(row.at(j), j);
+          if (at < CAP) {
+            A z;
+            if constexpr (FLAT) {
+              z = to_acc(reinterpret_cast<const T*>(slot + (q / VE) * 32)[q % VE]);
+              if (negate) z = -z;
+            } else {
+              z = row.at(j);
+            }
+            list[at] = Key<A>::of(z, j);
+          }
           in &= in - 1u;
         }
         count += __popc(b & team_lanes);
       }
     }
+    if (!early && more) fetch(first + step + team);
     if (__any_sync(0xffffffffu, t == lowest<A>())) {
       // masked scores by index: the first 2 top hold enough of them
       for (int j0 = 0; j0 < min(a.m, 2 * a.top); j0 += TEAM) {
@@ -602,27 +635,27 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int lo
     sums.template add<VE>(y, mine == neg_inf<A>() ? A(0) : mine, c);
   }
   int g = 0, in_group = 0;
+  // vectors behind the slice hold z = -inf; a step's vectors are read while the one before it
+  // is worked on
+  const uint4 fill = row.masked();
   const uint4* from = row.base + i0 + threadIdx.x;
-  for (int s = 0; s < steps; ++s, from += U * NT) {
-    A y[U * VE];
+  uint4 next[U];
+  auto fetch = [&](int s) {
     if ((s + 1) * (U * NT) <= i1 - i0) {
-      uint4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = load_keep(from + u * NT);
-#pragma unroll
-      for (int u = 0; u < U; ++u) row.values(w[u], y + u * VE);
+      for (int u = 0; u < U; ++u) next[u] = load_keep(from + s * (U * NT) + u * NT);
     } else {
       const int left = i1 - i0 - s * (U * NT) - static_cast<int>(threadIdx.x);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u * NT < left) {
-          row.values(load_keep(from + u * NT), y + u * VE);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) y[u * VE + e] = neg_inf<A>();
-        }
-      }
+      for (int u = 0; u < U; ++u) next[u] = u * NT < left ? load_keep(from + s * (U * NT) + u * NT) : fill;
     }
+  };
+  if (steps > 0) fetch(0);
+  for (int s = 0; s < steps; ++s) {
+    A y[U * VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row.values(next[u], y + u * VE);
+    if (s + 1 < steps) fetch(s + 1);
     A most;
     if constexpr (LISTS > 1) {
       A m4[U];
@@ -944,16 +977,28 @@ template <typename T> __global__ void __launch_bounds__(256) scores_grad_kernel(
 }
 
 // ------------------------------------------------------------------ launches
+// whether every row is whole 16-byte vectors
+template <typename T> static bool rows_are_vectors(const ScoreArgs<T>& a) {
+  return a.m % RowVecs<T>::VE == 0 &&
+         ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ld * sizeof(T))) & 15u) == 0;
+}
+
 template <typename T, int TEAM, int EPL> static cudaError_t scores_team(const ScoreArgs<T>& a, cudaStream_t st) {
-  constexpr int VE = RowVecs<T>::VE;
   const unsigned blocks =
-      static_cast<unsigned>(std::min<int64_t>((a.n * TEAM + 127) / 128, static_cast<int64_t>(num_sms()) * 20));
-  const bool flat =
-      a.m % VE == 0 && ((reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.ld * sizeof(T))) & 15u) == 0;
-  if (flat)
-    scores_team_kernel<T, TEAM, EPL, true><<<blocks, 128, 0, st>>>(a);
-  else
+      static_cast<unsigned>(std::min<int64_t>((a.n * TEAM + 127) / 128, static_cast<int64_t>(num_sms()) * 28));
+  constexpr size_t rows = 128 * EPL * sizeof(T);  // a row per team
+  if (rows_are_vectors(a)) {
+    if (rows > 32 * 1024 - 1) {  // near 48 KiB with the candidates
+      const cudaError_t e = cudaFuncSetAttribute(scores_team_kernel<T, TEAM, EPL, true>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rows));
+      if (e != cudaSuccess) return e;
+    }
+    scores_team_kernel<T, TEAM, EPL, true><<<blocks, 128, rows, st>>>(a);
+  } else if constexpr (EPL <= 32) {
     scores_team_kernel<T, TEAM, EPL, false><<<blocks, 128, 0, st>>>(a);
+  } else {
+    return cudaErrorInvalidValue;
+  }
   return cudaGetLastError();
 }
 
@@ -1015,11 +1060,12 @@ template <typename T> static cudaError_t scores_t(const ScoreJob& j, cudaStream_
   // a row in one team's registers where it fits; 8 lanes bound few alternatives well
   if (a.top <= 8 && a.m <= 64) return scores_team<T, 8, 8>(a, st);
   if (a.top <= 8 && a.m <= 256) return scores_team<T, 8, 32>(a, st);
+  if (a.top <= 16 && a.m <= 512 && a.m > 256) return scores_team<T, 16, 32>(a, st);
   if (a.m <= 256) return scores_team<T, 32, 8>(a, st);
   if (a.m <= 512) return scores_team<T, 32, 16>(a, st);
   if (a.m <= 1024) return scores_team<T, 32, 32>(a, st);
   if constexpr (sizeof(T) < 8)
-    if (a.m <= 2048 && a.n >= num_sms() * 4) return scores_team<T, 32, 64>(a, st);
+    if (a.m <= 2048 && a.n >= num_sms() * 4 && rows_are_vectors(a)) return scores_team<T, 32, 64>(a, st);
   if (a.m <= 8192 && a.n >= num_sms() * 8) return scores_block<T, 64>(a, st);
   if (a.n >= num_sms() * 4 && static_cast<int64_t>(a.m) * static_cast<int64_t>(sizeof(T)) <= 262144)
     return scores_block<T, 128>(a, st);
