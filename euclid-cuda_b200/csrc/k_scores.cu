@@ -392,7 +392,7 @@ __device__ __forceinline__ void copy_async_16(void* to, const void* from) {
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <typename T, int TEAM, int EPL, bool FLAT>
-__global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) == 8 ? 2 : 4) : (FLAT ? 7 : 5))
+__global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) == 8 ? 2 : 5) : (FLAT ? 7 : 5))
     scores_team_kernel(ScoreArgs<T> a) {
   using A = Acc<T>;
   constexpr int VE = FLAT ? RowVecs<T>::VE : 1, NV = EPL / VE, RPW = 32 / TEAM, CAP = kTeamCands<TEAM>;
@@ -746,17 +746,30 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int lo
           if (row.at(j) == neg_inf<A>()) add(neg_inf<A>(), j);
       __syncthreads();
       slow = hits_sh > kBlockHits;
-      if (!slow) {  // a warp per group of vectors, a lane per score
-        const int found = hits_sh;
-        for (int h = warp; h < found; h += W) {
-          const int q = static_cast<int>(hits[h] / NT), thread = static_cast<int>(hits[h] % NT);
-          for (int z = lane; z < per_group * (U * VE); z += 32) {
-            const int s = q * per_group + z / (U * VE), u = z / VE % U;
-            const int v = i0 + s * (U * NT) + u * NT + thread;
-            if (v >= i1) continue;
-            const int j = v * VE - row.off + z % VE;
-            const A y = row.at(j);
-            if (y >= bound) add(y, j);
+      if (!slow) {  // the groups' vectors over all threads, four reads in flight each
+        const int per_hit = per_group * U, all = hits_sh * per_hit;
+        for (int z0 = threadIdx.x; z0 < all; z0 += 4 * NT) {
+          uint4 w[4];
+          int v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[q] = i1;
+            const int z = z0 + q * NT;
+            if (z < all) {
+              const uint32_t hit = hits[z / per_hit];
+              const int in_hit = z % per_hit, s = static_cast<int>(hit / NT) * per_group + in_hit / U;
+              v[q] = i0 + s * (U * NT) + in_hit % U * NT + static_cast<int>(hit % NT);
+            }
+            w[q] = v[q] < i1 ? row.read(v[q]) : fill;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            A y[VE];
+            row.values(w[q], y);
+            if (max_of<A, VE>(y) < bound) continue;
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+              if (y[e] >= bound) add(y[e], v[q] * VE - row.off + e);
           }
         }
       }
