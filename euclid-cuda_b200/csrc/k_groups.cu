@@ -29,7 +29,9 @@ namespace euc {
 
 // ------------------------------------------------------------------ the sort
 constexpr int kBlockBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass of a block,
-constexpr int kMaxBins = 1537;    // and of three kernels (1048576 slots of 4000 labels: 50 us in two passes, 94 in one)
+constexpr int kMaxBins = 4609;    // and of three kernels: what shared memory holds per warp and bin
+constexpr int kManyBins = 1537;   // of more than kManySlots slots (262144 of 3000 labels: 22 us in one pass, 27 in
+constexpr int64_t kManySlots = 1 << 18;  // two; 1048576 of 4000: 94 in one, 50 in two)
 constexpr int kPassBits = 11;     // digits of a sort of several passes, at most
 
 struct SortOut {
@@ -351,7 +353,7 @@ static SortPlan sort_plan(int64_t n, int64_t k) {
   SortPlan p{};
   p.block = n <= kBlockSlots;
   p.tiles = static_cast<int>(((n + kTile - 1) / kTile + 3) / 4 * 4);
-  if (k + 1 <= (p.block ? kBlockBins : kMaxBins)) {
+  if (k + 1 <= (p.block ? kBlockBins : n <= kManySlots ? kMaxBins : kManyBins)) {
     p.passes = 1;
     p.bins = static_cast<int>(k + 1);
     return p;

@@ -55,7 +55,8 @@ template <> struct Key<float> {
     r.k = 0;
     return r;
   }
-  __device__ __forceinline__ float y() const { return value_of(static_cast<uint32_t>(k >> 32)); }
+  __device__ __forceinline__ uint32_t order() const { return static_cast<uint32_t>(k >> 32); }
+  __device__ __forceinline__ float y() const { return value_of(order()); }
   __device__ __forceinline__ int j() const { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
   __device__ __forceinline__ bool ahead(const Key& o) const { return k > o.k; }
   __device__ __forceinline__ Key other(int s) const {
@@ -79,6 +80,7 @@ template <> struct Key<double> {
     r.col = 0x7fffffff;
     return r;
   }
+  __device__ __forceinline__ unsigned long long order() const { return o; }
   __device__ __forceinline__ double y() const { return value_of(o); }
   __device__ __forceinline__ int j() const { return static_cast<int>(col); }
   __device__ __forceinline__ bool ahead(const Key& q) const { return o > q.o || (o == q.o && col < q.col); }
@@ -342,9 +344,11 @@ __device__ __forceinline__ void both(const Sums<double>& p, double& s, double& t
 // maxima that the softmax needs anyhow: the row is cut into lists of maxima (over the lanes),
 // and with q = ceil(top / lists) the smallest of the lists' q-th largest is reached by q of
 // every list.  The scores that reach it go to a candidate list in shared memory (in any
-// order), and a candidate's place is the number of candidates before it.  More candidates
-// than the list holds (many equal scores), or a NaN, take the plain way: the best one behind
-// the last one, `top` times.
+// order), and a candidate's place is the number of candidates before it.  Where they are more
+// than the list holds (sorted rows, say), a block takes the last place among those it holds
+// for a better bound; equal scores beyond that, and a NaN, take the plain way: the best one
+// behind the last one, `top` times.
+
 // The q-th largest over the team's lanes of each list, the smallest over the lists: q - 1
 // rounds strike each list's largest (and its equals, which only lowers the bound).  No NaN.
 // A row that is masked but for fewer scores gives the lowest finite number.
@@ -528,19 +532,33 @@ __global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) =
       }
     }
     if (__any_sync(0xffffffffu, slow)) {
+      // the best one behind the last one; after it the next equal one, if there is any, which
+      // is the first such score behind it
       Key<A> last = Key<A>::none();
+      int from = a.m;  // where the next equal one is looked for
       for (int k = 0; k < a.top; ++k) {
         Key<A> best = Key<A>::none();
-        for (int j = tl; j < a.m; j += TEAM) {
-          const Key<A> o = Key<A>::of(row.at(j), j);
-          if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
+        for (int j0 = from; __any_sync(0xffffffffu, j0 < a.m && best.order() == 0); j0 += TEAM) {
+          const int j = j0 + tl;
+          const bool equal = best.order() == 0 && j < a.m && order_of(row.at(j)) == last.order();
+          const unsigned b = __ballot_sync(0xffffffffu, equal) & team_lanes;
+          if (b != 0u) best = Key<A>::of(last.y(), j0 + (__ffs(b) - 1) % TEAM);
         }
+        if (__any_sync(0xffffffffu, best.order() == 0)) {
+          Key<A> other = Key<A>::none();
+          for (int j = tl; j < a.m; j += TEAM) {
+            const Key<A> o = Key<A>::of(row.at(j), j);
+            if ((k == 0 || last.ahead(o)) && o.ahead(other)) other = o;
+          }
 #pragma unroll
-        for (int s = TEAM / 2; s > 0; s >>= 1) {
-          const Key<A> o = best.other(s);
-          if (o.ahead(best)) best = o;
+          for (int s = TEAM / 2; s > 0; s >>= 1) {
+            const Key<A> o = other.other(s);
+            if (o.ahead(other)) other = o;
+          }
+          if (best.order() == 0) best = other;
         }
         last = best;
+        from = best.j() + 1;
         if (tl == 0 && slow && live) write_top(a, i, k, best, hi, L);
       }
     }
@@ -578,7 +596,7 @@ template <typename A> struct Part {  // one block's share of a row
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int log_cluster, int per_group) {
+__global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1) scores_block_kernel(ScoreArgs<T> a, int log_cluster, int per_group) {
   using A = Acc<T>;
   constexpr int VE = RowVecs<T>::VE, U = kBlockVecs, W = NT / 32, LISTS = W == 1 ? U : 1;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -605,6 +623,7 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int lo
   if (threadIdx.x == 0 && row.lo > 0 && v0 == 0) edge = 0;
   if (threadIdx.x == NT - 1 && row.hi < row.all && v1 == row.all && v0 < v1 && !(row.lo > 0 && row.all == 1)) edge = row.all - 1;
   if (threadIdx.x == 0) count_sh = hits_sh = 0;
+  __syncwarp();
   if (cluster > 1) cluster_arrive();  // waited for before the first store to another block
 
   // the label's score, read ahead of its use
@@ -725,7 +744,7 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int lo
   Key<A>* list = lists[rank];
   if (want > 0) {
     bool slow = hi != hi;
-    if (!slow) {
+    while (!slow) {
       auto add = [&](A y, int j) {
         const int at = atomicAdd(&count_sh, 1);
         if (at < kBlockCands) cands[at] = Key<A>::of(y, j);
@@ -745,64 +764,89 @@ __global__ void __launch_bounds__(NT) scores_block_kernel(ScoreArgs<T> a, int lo
         for (int j = j0 + static_cast<int>(threadIdx.x); j < min(j1, j0 + 2 * want); j += NT)
           if (row.at(j) == neg_inf<A>()) add(neg_inf<A>(), j);
       __syncthreads();
-      slow = hits_sh > kBlockHits;
-      if (!slow) {  // the groups' vectors over all threads, four reads in flight each
-        const int per_hit = per_group * U, all = hits_sh * per_hit;
-        for (int z0 = threadIdx.x; z0 < all; z0 += 4 * NT) {
-          uint4 w[4];
-          int v[4];
+      // the groups' vectors over all threads, R reads in flight each
+      constexpr int R = VE == 8 ? 2 : 4;
+      const int per_hit = per_group * U, all = min(hits_sh, kBlockHits) * per_hit;
+      for (int z0 = threadIdx.x; z0 < all; z0 += R * NT) {
+        uint4 w[R];
+        int v[R];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            v[q] = i1;
-            const int z = z0 + q * NT;
-            if (z < all) {
-              const uint32_t hit = hits[z / per_hit];
-              const int in_hit = z % per_hit, s = static_cast<int>(hit / NT) * per_group + in_hit / U;
-              v[q] = i0 + s * (U * NT) + in_hit % U * NT + static_cast<int>(hit % NT);
-            }
-            w[q] = v[q] < i1 ? row.read(v[q]) : fill;
+        for (int q = 0; q < R; ++q) {
+          v[q] = i1;
+          const int z = z0 + q * NT;
+          if (z < all) {
+            const uint32_t hit = hits[z / per_hit];
+            const int in_hit = z % per_hit, s = static_cast<int>(hit / NT) * per_group + in_hit / U;
+            v[q] = i0 + s * (U * NT) + in_hit % U * NT + static_cast<int>(hit % NT);
           }
+          w[q] = v[q] < i1 ? row.read(v[q]) : fill;
+        }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            A y[VE];
-            row.values(w[q], y);
-            if (max_of<A, VE>(y) < bound) continue;
+        for (int q = 0; q < R; ++q) {
+          A y[VE];
+          row.values(w[q], y);
+          if (max_of<A, VE>(y) < bound) continue;
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-              if (y[e] >= bound) add(y[e], v[q] * VE - row.off + e);
-          }
+          for (int e = 0; e < VE; ++e)
+            if (y[e] >= bound) add(y[e], v[q] * VE - row.off + e);
         }
       }
       __syncthreads();
-      slow |= count_sh > kBlockCands;
-    }
-    if (!slow) {
-      const int count = count_sh;
+      const int count = min(count_sh, kBlockCands);
+      const bool whole = count_sh <= kBlockCands && hits_sh <= kBlockHits;
       for (int q = threadIdx.x; q < count; q += NT) {
         const Key<A> me = cands[q];
         const int place = place_of(cands, count, me);
         if (place < want) list[place] = me;
       }
-    } else {
+      if (whole) break;
+      // too many for the list: the last place among those it holds bounds the row's better,
+      // unless they are all equal
+      __syncthreads();
+      const A better = list[want - 1].y();
+      slow = !(better > bound);
+      bound = better;
+      __syncthreads();
+      if (threadIdx.x == 0) count_sh = hits_sh = 0;
+      __syncthreads();
+    }
+    if (slow) {
+      // the best one behind the last one; after it the next equal one, if there is any, which
+      // is the first such score behind it
       Key<A> last = Key<A>::none();
+      int from = j1;  // where the next equal one is looked for
       for (int k = 0; k < want; ++k) {
         Key<A> best = Key<A>::none();
-        for (int j = j0 + static_cast<int>(threadIdx.x); j < j1; j += NT) {
-          const Key<A> o = Key<A>::of(row.at(j), j);
-          if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
-        }
+        for (int s = from; s < j1 && best.order() == 0; s += NT) {
+          const int j = s + static_cast<int>(threadIdx.x);
+          const bool equal = j < j1 && order_of(row.at(j)) == last.order();
+          const unsigned b = __ballot_sync(0xffffffffu, equal);
+          __syncthreads();
+          if (lane == 0) cands[warp] = b != 0u ? Key<A>::of(last.y(), s + warp * 32 + __ffs(b) - 1) : Key<A>::none();
+          __syncthreads();
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-          const Key<A> o = best.other(s);
-          if (o.ahead(best)) best = o;
+          for (int w = 0; w < W; ++w)
+            if (cands[w].ahead(best)) best = cands[w];
         }
-        __syncthreads();
-        if (lane == 0) cands[warp] = best;
-        __syncthreads();
+        if (best.order() == 0) {
+          for (int j = j0 + static_cast<int>(threadIdx.x); j < j1; j += NT) {
+            const Key<A> o = Key<A>::of(row.at(j), j);
+            if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
+          }
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-          if (cands[w].ahead(best)) best = cands[w];
+          for (int s = 16; s > 0; s >>= 1) {
+            const Key<A> o = best.other(s);
+            if (o.ahead(best)) best = o;
+          }
+          __syncthreads();
+          if (lane == 0) cands[warp] = best;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (cands[w].ahead(best)) best = cands[w];
+        }
         last = best;
+        from = best.j() + 1;
         if (threadIdx.x == 0) list[k] = best;
       }
     }
@@ -876,7 +920,7 @@ template <typename T> struct ScoreGradArgs {
 // scale g_l more at the label: per score a subtraction, two fused multiply-adds, one
 // exponential and a product, fp32 in pairs.  One warp per (row, kGradVecs 16-byte vectors a
 // lane) of the output, whose alignment decides where the vectors begin; scores whose row
-// starts elsewhere in its 16 bytes are read element by element.
+// starts elsewhere in its 16 bytes are put together from two aligned reads.
 constexpr int kGradVecs = 4;
 
 template <typename A> struct GradRow {
@@ -945,14 +989,17 @@ template <typename T> __global__ void __launch_bounds__(256) scores_grad_kernel(
   } else {
 #pragma unroll
     for (int u = 0; u < kGradVecs; ++u) {
-      Vec<T, VE> v;
-      v.raw = raw_zero<uint4>();
+      const int j = j0 + u * 32 * VE;
+      if (j >= 0 && j + VE <= a.m) {
+        w[u] = load_any_16(x + j, a.x, a.x + (a.n - 1) * a.ld + a.m);
+      } else {
+        Vec<T, VE> v;
+        v.raw = raw_zero<uint4>();
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const int j = j0 + u * 32 * VE + e;
-        if (j >= 0 && j < a.m) v.e[e] = x[j];
+        for (int e = 0; e < VE; ++e)
+          if (j + e >= 0 && j + e < a.m) v.e[e] = x[j + e];
+        w[u] = v.raw;
       }
-      w[u] = v.raw;
     }
   }
   const A hi = a.stats[3 * i], L = a.stats[3 * i + 1], H = a.stats[3 * i + 2];

@@ -9,7 +9,8 @@
 namespace euc {
 
 constexpr int64_t kMaxIndex = 0x7ffffffell;  // sorted positions, slots and labels are int32
-constexpr int64_t kMaxScores = 1ll << 30;    // a row's elements and vectors are counted in int32
+constexpr int64_t kMaxScores = 1ll << 30;    // a row's elements and vectors are counted in int32,
+constexpr int64_t kMaxDim = 1ll << 30;       // in every operator
 constexpr int kMaxTop = 32;
 
 static int done(cudaError_t e, const char* where) {
@@ -30,7 +31,7 @@ static int no_device() {
 static int rows_shape(int64_t n, int64_t p, int64_t dim) {
   if (n < 0 || p < 0 || dim < 0) return set_error(EUC_ERR_SHAPE, "negative size");
   if (n > kMaxIndex || p > kMaxIndex || (p > 0 && n > kMaxIndex / p)) return set_error(EUC_ERR_SHAPE, "too many slots");
-  if (dim > kMaxIndex) return set_error(EUC_ERR_SHAPE, "dim too large");
+  if (dim > kMaxDim) return set_error(EUC_ERR_SHAPE, "dim too large");
   return EUC_OK;
 }
 
@@ -182,7 +183,7 @@ int euc_codebook_lookup(int row_type, const void* C, int64_t k, const void* labe
                         int64_t dim, double scale, void* out, void* stream) {
   if (int rc = bad_type(row_type)) return rc;
   if (n < 0 || k < 0 || dim < 0) return set_error(EUC_ERR_SHAPE, "negative size");
-  if (dim > kMaxIndex || (dim > 0 && n > (int64_t(1) << 62) / dim)) return set_error(EUC_ERR_SHAPE, "shape too large");
+  if (dim > kMaxDim || (dim > 0 && n > (int64_t(1) << 62) / dim)) return set_error(EUC_ERR_SHAPE, "shape too large");
   if (int rc = no_device()) return rc;
   if (n == 0 || dim == 0) return EUC_OK;
   if (!labels || !out || (k > 0 && !C)) return set_error(EUC_ERR_ARG, "null pointer");

@@ -55,6 +55,43 @@ template <> __device__ __forceinline__ uint2 raw_zero<uint2>() { return make_uin
 template <> __device__ __forceinline__ uint32_t raw_zero<uint32_t>() { return 0u; }
 template <> __device__ __forceinline__ unsigned short raw_zero<unsigned short>() { return 0; }
 
+template <int BYTES> struct BitsOf;
+template <> struct BitsOf<2> { using type = unsigned short; };
+template <> struct BitsOf<4> { using type = uint32_t; };
+template <> struct BitsOf<8> { using type = unsigned long long; };
+
+// The 16 bytes at any address that T's alignment allows, from the two aligned 16-byte words
+// that hold them (neighbouring lanes share them, so the second comes from L1); element by
+// element where one of the words is not inside [begin, end).
+template <typename T>
+__device__ __forceinline__ uint4 load_any_16(const T* p, const void* begin, const void* end) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), shift = at & 15u;
+  const uint4* w = reinterpret_cast<const uint4*>(at - shift);
+  if (shift == 0) return load_keep(w);
+  if (static_cast<const void*>(w) < begin || static_cast<const void*>(w + 2) > end) {
+    using Bits = typename BitsOf<sizeof(T)>::type;
+    union {
+      uint4 raw;
+      Bits e[16 / sizeof(T)];
+    } v;
+#pragma unroll
+    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) v.e[e] = reinterpret_cast<const Bits*>(p)[e];
+    return v.raw;
+  }
+  const uint4 a = load_keep(w), b = load_keep(w + 1);
+  const unsigned bits = static_cast<unsigned>(shift & 3u) * 8u;
+  auto pick = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4) {
+    return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                      __funnelshift_r(w3, w4, bits));
+  };
+  switch (shift >> 2) {  // the same for all vectors of a row
+    case 0: return pick(a.x, a.y, a.z, a.w, b.x);
+    case 1: return pick(a.y, a.z, a.w, b.x, b.y);
+    case 2: return pick(a.z, a.w, b.x, b.y, b.z);
+    default: return pick(a.w, b.x, b.y, b.z, b.w);
+  }
+}
+
 // Bytes of the widest vector that every row of `row_bytes` starts and ends on, given the
 // OR of the buffers' addresses: 16, 8, 4 or 2 (elements are of 2 bytes at least).
 inline int row_vec_bytes(int64_t row_bytes, uintptr_t addresses) {

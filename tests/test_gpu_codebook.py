@@ -63,7 +63,7 @@ def check(C, G, lab, scale):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["even", "drop", "one", "none", "skew"])
 @pytest.mark.parametrize("n,k,d", [(1, 1, 1), (3, 5, 2048), (100, 7, 33), (1000, 50, 77), (5000, 300, 64),
-                                   (700, 5000, 16), (2100, 1, 130)])
+                                   (700, 5000, 16), (2100, 1, 130), (90, 40, 515), (33, 9, 1001)])
 def test_lookup_and_gradient(n, k, d, kind, dtype):
     g = gen(n + k + d)
     C = torch.randn(k, d, generator=g, device="cuda", dtype=torch.float64).to(dtype)

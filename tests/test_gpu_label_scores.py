@@ -90,6 +90,24 @@ def test_equal_scores_go_by_index(dtype, m, top):
     check(x, torch.tensor([0, m - 1, m // 2], device="cuda"), -2.0, top)
 
 
+@pytest.mark.parametrize("n,m,top", [(5, 60, 8), (5, 250, 30), (3, 1000, 20), (3, 2000, 8), (700, 2000, 5),
+                                     (2, 9000, 32), (1300, 3000, 8), (1300, 9001, 4), (2, 100003, 32), (1, 131072, 20)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_sorted_and_stepped_rows(n, m, top, dtype):
+    """Rows whose best scores lie together: rising, falling, in steps of equal ones, and nearly
+    all equal; far more scores than the candidates' list holds reach any early bound."""
+    ramp = torch.arange(m, device="cuda", dtype=torch.float32)
+    rows = [ramp / m, -ramp / m, (ramp / 700).floor(), -(ramp / 700).floor(), torch.zeros_like(ramp),
+            (ramp % 2), torch.where(ramp == m // 2, 1.0, 0.0)]
+    x = torch.stack([rows[i % len(rows)] for i in range(n)]).to(dtype)
+    lab = torch.arange(n, device="cuda") % m
+    check(x[:7], lab[:7], 1.0, top, grads=False)
+    r, few = label_log_probs(x, lab, 1.0, top), label_log_probs(x[:7], lab[:7], 1.0, top)
+    for i in range(0, n, 97):  # a row among many as a row among few, whichever kernel takes it
+        if i % 7 < min(7, n):
+            assert torch.equal(r.top_labels[i], few.top_labels[i % 7])
+
+
 def test_zeros_of_both_signs_are_equal():
     x = torch.zeros(2, 100, device="cuda")
     x[0, ::2] = -0.0
