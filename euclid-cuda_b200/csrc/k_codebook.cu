@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
 // neighbouring vectors, its other threads every so-manyth chunk, and whose sums are added in
 // a fixed order.
 constexpr int kLongChunks = 64;
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512;
 constexpr int kJoinCandidates = 4;  // multiples of kLongChunks that a block looks at
 
 // sum over chunks [c, c1], every `step`-th, of the label that starts at position lo
@@ -344,37 +344,40 @@ __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(GradArgs a, int
     join_long<T, N>(a, blockIdx.x, scale, part, out);
     return;
   }
-  // SUB 4: a warp takes eight neighbouring vectors at one border, its four lanes of a vector
-  // every fourth chunk; SUB 1 (rows of fewer vectors): a thread per vector and border
+  // SUB 4: a warp takes 32 neighbouring vectors at one border, eight at a time, its four lanes
+  // of a vector every fourth chunk; SUB 1 (rows of fewer vectors): a thread per vector and border
   constexpr int VW = 32 / SUB;
-  const int lane = threadIdx.x & 31, sub = lane / VW;
+  const int lane = threadIdx.x & 31, sub = SUB == 1 ? 0 : lane / VW;
   const int64_t t = static_cast<int64_t>(blockIdx.x - long_blocks) * blockDim.x + threadIdx.x;
-  const int64_t unit = SUB == 1 ? t : t >> 5, tiles = SUB == 1 ? a.nv : (a.nv + VW - 1) / VW;
+  const int64_t unit = SUB == 1 ? t : t >> 5, tiles = SUB == 1 ? a.nv : (a.nv + 31) / 32;
   const int64_t border =
       1 + (unit < 0x80000000ll ? static_cast<uint32_t>(unit) / static_cast<uint32_t>(tiles) : unit / tiles);
-  const int64_t tile = unit - (border - 1) * tiles;
-  const int64_t v = SUB == 1 ? tile : tile * VW + lane % VW, at = border * a.seg;
+  const int64_t tile = unit - (border - 1) * tiles, at = border * a.seg;
   if (at >= min(a.n, static_cast<int64_t>(a.offsets[a.k]))) return;
   const int64_t c = a.labels[at];
   if (c < 0 || c >= a.k || a.labels[at - 1] != c) return;
   const int64_t lo = max(0, a.offsets[c]), hi = min(a.n, static_cast<int64_t>(a.offsets[c + 1]));
   const int64_t c0 = lo / a.seg, c1 = (hi - 1) / a.seg;
   if (c0 != border - 1 || c1 - c0 >= kLongChunks) return;  // an earlier border's, or a block's
-  A acc[N];
+  // (a warp of SUB 4 is at one border: all of its lanes are here)
+  for (int q = 0; q < SUB; ++q) {
+    const int64_t v = SUB == 1 ? tile : tile * 32 + q * VW + lane % VW;
+    A acc[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = A(0);
-  if (v < a.nv) add_parts<A, N>(part, c0 + (SUB == 1 ? 0 : sub), c1, SUB, lo, a.seg, a.nv, v, acc);
-  if constexpr (SUB > 1) {  // (the warp is at one border: all of its lanes are here)
+    for (int e = 0; e < N; ++e) acc[e] = A(0);
+    if (v < a.nv) add_parts<A, N>(part, c0 + sub, c1, SUB, lo, a.seg, a.nv, v, acc);
+    if constexpr (SUB > 1) {
 #pragma unroll
-    for (int s = VW; s < 32; s <<= 1)
+      for (int s = VW; s < 32; s <<= 1)
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], s);
+        for (int e = 0; e < N; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], s);
+    }
+    if (sub != 0 || v >= a.nv) continue;
+    V o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
+    store_once(reinterpret_cast<Raw*>(out) + c * a.nv + v, o.raw);
   }
-  if ((SUB > 1 && sub != 0) || v >= a.nv) return;
-  V o;
-#pragma unroll
-  for (int e = 0; e < N; ++e) o.e[e] = from_acc<T>(scale * acc[e]);
-  store_once(reinterpret_cast<Raw*>(out) + c * a.nv + v, o.raw);
 }
 
 // ------------------------------------------------------------------ launches
@@ -413,6 +416,8 @@ static cudaError_t lookup_go(const T* C, int64_t k, const TL* labels, int64_t n,
   if (n * nv <= static_cast<int64_t>(num_sms()) * 2048) return wide(lookup_kernel<T, N, TL, 1, 1, true>, 1, 1);
   if (nv <= 32) return wide(lookup_kernel<T, N, TL, 4, 1, true>, 4, 1);
   if (nv <= 64) return wide(lookup_kernel<T, N, TL, 2, 2, true>, 2, 2);
+  // (57934 rows of 554 fp32, 8 bytes at a time: 44 us with two vectors a lane)
+  if (N * sizeof(T) < 16) return wide(lookup_kernel<T, N, TL, 1, 4, true>, 1, 4);
   return wide(lookup_kernel<T, N, TL, 1, 2, true>, 1, 2);
 }
 
@@ -443,7 +448,7 @@ static cudaError_t grad_n(const T* G, GradArgs a, int64_t dim, double scale, T* 
     if (e != cudaSuccess) return e;
     // four lanes a vector where the row has eight vectors to fill the warp's others
     const bool four = a.nv >= 8;
-    const int64_t threads = (a.chunks - 1) * (four ? (a.nv + 7) / 8 * 32 : a.nv);
+    const int64_t threads = (a.chunks - 1) * (four ? (a.nv + 31) / 32 * 32 : a.nv);
     const unsigned g = static_cast<unsigned>(longs + (threads + kJoinThreads - 1) / kJoinThreads);
     return four ? launch_after(true, grad_join_kernel<T, N, 4>, g, kJoinThreads, 0, st, a, longs, s, part, out)
                 : launch_after(true, grad_join_kernel<T, N, 1>, g, kJoinThreads, 0, st, a, longs, s, part, out);
