@@ -15,8 +15,8 @@
 // keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit counters per warp
 // and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in 2.7 us.  More take
 // three kernels a pass (histograms of tiles, scan of each bin over the tiles, scatter through
-// shared memory so that a bin's run is stored together), 131072 slots of 128 labels in 8.3
-// us, 8192 of 256 in 8.5 (one block 23); one cluster of 8 blocks took 54 for them, since eight SMs scatter no faster.  The sort
+// shared memory so that a bin's run is stored together), 131072 slots of 128 labels in 6.7
+// us, 8192 of 256 in 7.1 (one block 23); one cluster of 8 blocks took 54 for them, since eight SMs scatter no faster.  The sort
 // moves 4 to 8 bytes a slot where the rows move kilobytes; the row kernels are bound by HBM,
 // and read and write every row once: a row's copies are written from registers after one
 // read, its weighted sum is formed from p reads.
@@ -98,10 +98,9 @@ struct BlockSort {
   uint32_t *keys[2], *slots[2];  // between passes
 };
 
-constexpr int kBlockItems = 2;
-constexpr int64_t kBlockSlots = 1024 * kBlockItems;
+constexpr int64_t kBlockSlots = 1024;
 
-template <typename TL, int ITEMS>
+template <typename TL>
 __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__ in, BlockSort a, SortOut o) {
   extern __shared__ uint32_t sm[];
   __shared__ uint32_t warp_sums[32];
@@ -110,24 +109,19 @@ __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__
   uint32_t* start = sm;  // [bins] first position of the digit
   unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + a.bins);  // [warps][bins]
   unsigned short* mine = cnt + warp * a.bins;
-  const int base = warp * (32 * ITEMS) + lane;
+  const int s = static_cast<int>(threadIdx.x);
   for (int pass = 0; pass < a.passes; ++pass) {
     const bool last = pass == a.passes - 1;
     const int shift = pass * a.bits;
     const uint32_t mask = a.passes == 1 ? 0xffffffffu : (1u << a.bits) - 1u;
     const uint32_t* from_keys = a.keys[(pass + 1) & 1];
     const uint32_t* from_slots = a.slots[(pass + 1) & 1];
-    uint32_t key[ITEMS], digit[ITEMS];
-    unsigned short rank[ITEMS];
-#pragma unroll
-    for (int u = 0; u < ITEMS; ++u) {
-      const int s = base + u * 32;
-      key[u] = s >= a.n ? 0u : pass == 0 ? key_of(in[s], a.k) : __ldcg(from_keys + s);
-      digit[u] = s >= a.n ? 0xffffffffu : (key[u] >> shift) & mask;
-    }
+    const uint32_t key = s >= a.n ? 0u : pass == 0 ? key_of(in[s], a.k) : __ldcg(from_keys + s);
+    const uint32_t digit[1] = {s >= a.n ? 0xffffffffu : (key >> shift) & mask};
+    unsigned short rank[1];
     for (int c = threadIdx.x; c < a.bins * warps; c += blockDim.x) cnt[c] = 0;
     __syncthreads();
-    warp_ranks<ITEMS>(digit, rank, mine, lane);
+    warp_ranks<1>(digit, rank, mine, lane);
     __syncthreads();
     for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
       uint32_t run = 0;
@@ -142,19 +136,16 @@ __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__
     block_scan(start, a.bins, warp_sums);
     if (last && o.offsets)
       for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
-#pragma unroll
-    for (int u = 0; u < ITEMS; ++u) {
-      const int s = base + u * 32;
-      if (s >= a.n) continue;
-      const uint32_t pos = start[digit[u]] + mine[digit[u]] + rank[u];
+    if (s < a.n) {
+      const uint32_t pos = start[digit[0]] + mine[digit[0]] + rank[0];
       const uint32_t slot = pass == 0 ? static_cast<uint32_t>(s) : __ldcg(from_slots + s);
       if (last) {
-        const bool kept = key[u] < a.k;
+        const bool kept = key < a.k;
         o.order[pos] = kept ? static_cast<int32_t>(slot) : -1;
-        o.labels[pos] = kept ? static_cast<int32_t>(key[u]) : -1;
+        o.labels[pos] = kept ? static_cast<int32_t>(key) : -1;
         o.position[slot] = kept ? static_cast<int32_t>(pos) : -1;
       } else {
-        a.keys[pass & 1][pos] = key[u];
+        a.keys[pass & 1][pos] = key;
         a.slots[pass & 1][pos] = slot;
       }
     }
@@ -163,10 +154,8 @@ __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__
 }
 
 // ---- three kernels a pass
-constexpr int kTileWarps = 16;
-constexpr int kTileItems = 4;
-constexpr int kTile = kTileWarps * 32 * kTileItems;  // 2048 slots, so 16 bits index one of them
-
+// A tile is WARPS x 32 x ITEMS slots (at most 4096: 16 bits index one of them), sorted by a
+// block of WARPS warps.
 struct SortPass {
   int64_t n;
   uint32_t k;  // keys lie in [0, k]; k marks a dropped slot
@@ -183,23 +172,23 @@ template <typename TL, bool FIRST> __device__ __forceinline__ uint32_t load_key(
   else return static_cast<uint32_t>(in[s]);
 }
 
-template <typename TL, bool FIRST>
-__global__ void __launch_bounds__(kTileWarps * 32) sort_hist_kernel(const TL* __restrict__ in, SortPass a) {
+template <typename TL, bool FIRST, int WARPS, int ITEMS>
+__global__ void __launch_bounds__(WARPS * 32) sort_hist_kernel(const TL* __restrict__ in, SortPass a) {
   extern __shared__ uint32_t cnt[];
   let_next_start();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) cnt[c] = 0u;
   if (!FIRST) wait_for_previous();
   __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x;
-  uint32_t key[kTileItems];
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (WARPS * 32 * ITEMS) + threadIdx.x;
+  uint32_t key[ITEMS];
 #pragma unroll
-  for (int u = 0; u < kTileItems; ++u) {
-    const int64_t s = base + u * (kTileWarps * 32);
+  for (int u = 0; u < ITEMS; ++u) {
+    const int64_t s = base + u * (WARPS * 32);
     key[u] = s < a.n ? load_key<TL, FIRST>(in, s, a.k) : 0u;
   }
 #pragma unroll
-  for (int u = 0; u < kTileItems; ++u)
-    if (base + u * (kTileWarps * 32) < a.n) atomicAdd(&cnt[(key[u] >> a.shift) & a.mask], 1u);
+  for (int u = 0; u < ITEMS; ++u)
+    if (base + u * (WARPS * 32) < a.n) atomicAdd(&cnt[(key[u] >> a.shift) & a.mask], 1u);
   __syncthreads();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {
     uint32_t* row = a.T + static_cast<int64_t>(c) * a.tiles;
@@ -249,39 +238,39 @@ __global__ void __launch_bounds__(256) sort_tiles_kernel(SortPass a) {
   if (lane == 0) a.total[bin] = run;
 }
 
-template <typename TL, bool FIRST, bool LAST>
-__global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL* __restrict__ in,
+template <typename TL, bool FIRST, bool LAST, int WARPS, int ITEMS>
+__global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __restrict__ in,
                                                                       const uint32_t* __restrict__ in_slots,
                                                                       SortPass a, SortOut o) {
   extern __shared__ uint32_t sm[];
-  __shared__ uint32_t warp_sums[kTileWarps];
+  __shared__ uint32_t warp_sums[WARPS];
   uint32_t* start = sm;                  // [bins] global position of the tile's first slot of the bin,
   uint32_t* local = sm + a.bins;         // [bins] less its position in the tile
-  uint32_t* stage = sm + 2 * a.bins;     // [kTile] digit and slot, in the tile's order
-  unsigned short* cnt = reinterpret_cast<unsigned short*>(stage + kTile);  // [warps][bins]
+  uint32_t* stage = sm + 2 * a.bins;     // [tile] digit and slot, in the tile's order
+  unsigned short* cnt = reinterpret_cast<unsigned short*>(stage + (WARPS * 32 * ITEMS));  // [warps][bins]
   let_next_start();
-  for (int c = threadIdx.x; c < a.bins * (kTileWarps / 2); c += blockDim.x) reinterpret_cast<uint32_t*>(cnt)[c] = 0u;
+  for (int c = threadIdx.x; c < a.bins * (WARPS / 2); c += blockDim.x) reinterpret_cast<uint32_t*>(cnt)[c] = 0u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned short* mine = cnt + warp * a.bins;
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int first = warp * (32 * kTileItems) + lane;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) * (WARPS * 32 * ITEMS);
+  const int first = warp * (32 * ITEMS) + lane;
   // the ranks within the tile need the labels alone (of a first pass: what came before the
   // sort), so they are formed while the histograms are still being summed
   if (!FIRST) wait_for_previous();
-  uint32_t digit[kTileItems];
-  unsigned short rank[kTileItems];
+  uint32_t digit[ITEMS];
+  unsigned short rank[ITEMS];
 #pragma unroll
-  for (int u = 0; u < kTileItems; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t s = tile + first + u * 32;
     digit[u] = s < a.n ? (load_key<TL, FIRST>(in, s, a.k) >> a.shift) & a.mask : 0xffffffffu;
   }
   __syncthreads();
-  warp_ranks<kTileItems>(digit, rank, mine, lane);
+  warp_ranks<ITEMS>(digit, rank, mine, lane);
   __syncthreads();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
     uint32_t run = 0;
 #pragma unroll
-    for (int w = 0; w < kTileWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const unsigned short t = cnt[w * a.bins + c];
       cnt[w * a.bins + c] = static_cast<unsigned short>(run);
       run += t;
@@ -300,7 +289,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
     start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] - local[c];
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kTileItems; ++u)
+  for (int u = 0; u < ITEMS; ++u)
     if (digit[u] != 0xffffffffu) {
       const uint32_t l = local[digit[u]] + mine[digit[u]] + rank[u];
       stage[l] = (digit[u] << 16) | static_cast<uint32_t>(first + u * 32);
@@ -308,7 +297,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) sort_scatter_kernel(const TL*
       if (FIRST && LAST) o.position[tile + first + u * 32] = digit[u] < a.k ? static_cast<int32_t>(start[digit[u]] + l) : -1;
     }
   __syncthreads();
-  const int here = static_cast<int>(min(static_cast<int64_t>(kTile), a.n - tile));
+  const int here = static_cast<int>(min(static_cast<int64_t>((WARPS * 32 * ITEMS)), a.n - tile));
   for (int l = threadIdx.x; l < here; l += blockDim.x) {
     const uint32_t w = stage[l], d = w >> 16;
     const int64_t s = tile + (w & 0xffffu);
@@ -346,16 +335,28 @@ static inline size_t al(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct SortPlan {
   int passes, bits, bins, tiles;
+  int warps, items;  // of a tile
   bool block;
 };
+
+// Tiles: small ones fill the SMs, and are cheap to begin while the bins are few; large ones
+// leave fewer histograms to add up (131072 slots of 128 labels: 6.7, 8.3 and 11.0 us with
+// 8 x 4, 16 x 4 and 16 x 8; 65536 of 1024: 13.9, 14.9, 18.2; 1048576 of 1024: 41, 35, 27).
+static void set_tiles(SortPlan& p, int64_t n) {
+  const bool many = n > (1 << 19);
+  p.warps = !many && p.bins <= 1025 ? 8 : 16;
+  p.items = many ? 8 : 4;
+  const int tile = p.warps * 32 * p.items;
+  p.tiles = static_cast<int>(((n + tile - 1) / tile + 3) / 4 * 4);
+}
 
 static SortPlan sort_plan(int64_t n, int64_t k) {
   SortPlan p{};
   p.block = n <= kBlockSlots;
-  p.tiles = static_cast<int>(((n + kTile - 1) / kTile + 3) / 4 * 4);
   if (k + 1 <= (p.block ? kBlockBins : n <= kManySlots ? kMaxBins : kManyBins)) {
     p.passes = 1;
     p.bins = static_cast<int>(k + 1);
+    set_tiles(p, n);
     return p;
   }
   int bits = 1;
@@ -363,6 +364,7 @@ static SortPlan sort_plan(int64_t n, int64_t k) {
   p.passes = (bits + kPassBits - 1) / kPassBits;
   p.bits = (bits + p.passes - 1) / p.passes;
   p.bins = 1 << p.bits;
+  set_tiles(p, n);
   return p;
 }
 
@@ -383,39 +385,43 @@ static cudaError_t more_smem(const void* kernel, size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
-template <typename TL, int ITEMS>
+template <typename TL>
 static cudaError_t sort_block(const TL* in, const BlockSort& a, const SortOut& o, cudaStream_t st) {
-  const int nt = ((a.n + ITEMS - 1) / ITEMS + 31) / 32 * 32;
+  const int nt = (a.n + 31) / 32 * 32;
   const size_t smem = static_cast<size_t>(a.bins) * (4 + 2 * (nt / 32));
-  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_block_kernel<TL, ITEMS>), smem);
+  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_block_kernel<TL>), smem);
   if (e != cudaSuccess) return e;
-  sort_block_kernel<TL, ITEMS><<<1, nt, smem, st>>>(in, a, o);
+  sort_block_kernel<TL><<<1, nt, smem, st>>>(in, a, o);
   return cudaGetLastError();
 }
 
-template <typename TL, bool FIRST, bool LAST>
-static cudaError_t sort_pass(const TL* in, const uint32_t* in_slots, const SortPass& a, const SortOut& o,
-                             cudaStream_t st) {
-  const size_t sm = static_cast<size_t>(a.bins) * (8 + 2 * kTileWarps) + kTile * 4;
-  cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_scatter_kernel<TL, FIRST, LAST>), sm);
+template <typename TL, bool FIRST, bool LAST, int WARPS, int ITEMS>
+static cudaError_t sort_pass_t(const TL* in, const uint32_t* in_slots, const SortPass& a, const SortOut& o,
+                               cudaStream_t st) {
+  constexpr int TILE = WARPS * 32 * ITEMS;
+  const auto hist = sort_hist_kernel<TL, FIRST, WARPS, ITEMS>;
+  const auto scatter = sort_scatter_kernel<TL, FIRST, LAST, WARPS, ITEMS>;
+  const size_t sm = static_cast<size_t>(a.bins) * (8 + 2 * WARPS) + TILE * 4;
+  cudaError_t e = more_smem(reinterpret_cast<const void*>(scatter), sm);
   if (e != cudaSuccess) return e;
-  const unsigned tiles = static_cast<unsigned>((a.n + kTile - 1) / kTile);
+  const unsigned tiles = static_cast<unsigned>((a.n + TILE - 1) / TILE);
   // Each kernel may start while the one before it runs, if all their blocks fit beside one
   // another with little shared memory: 131072 slots of 128 labels take 8.1 us so, and 11.4
   // one after another; but 1048576 slots of 1024 labels 40 us, and 33 one after another.
   const bool early = a.bins <= 512 && static_cast<int>(tiles) <= num_sms();
-  if (FIRST || !early) {
-    sort_hist_kernel<TL, FIRST><<<tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st>>>(in, a);
-    e = cudaGetLastError();
-  } else {
-    e = launch_after(true, sort_hist_kernel<TL, FIRST>, tiles, kTileWarps * 32, static_cast<size_t>(a.bins) * 4, st, in,
-                     a);
-  }
+  e = launch_after(!FIRST && early, hist, tiles, WARPS * 32, static_cast<size_t>(a.bins) * 4, st, in, a);
   if (e == cudaSuccess)
     e = launch_after(early, sort_tiles_kernel, static_cast<unsigned>((a.bins + 7) / 8), 256, 0, st, a);
-  if (e == cudaSuccess)
-    e = launch_after(early, sort_scatter_kernel<TL, FIRST, LAST>, tiles, kTileWarps * 32, sm, st, in, in_slots, a, o);
+  if (e == cudaSuccess) e = launch_after(early, scatter, tiles, WARPS * 32, sm, st, in, in_slots, a, o);
   return e;
+}
+
+template <typename TL, bool FIRST, bool LAST>
+static cudaError_t sort_pass(const SortPlan& p, const TL* in, const uint32_t* in_slots, const SortPass& a,
+                             const SortOut& o, cudaStream_t st) {
+  if (p.items == 8) return sort_pass_t<TL, FIRST, LAST, 16, 8>(in, in_slots, a, o, st);
+  if (p.warps == 8) return sort_pass_t<TL, FIRST, LAST, 8, 4>(in, in_slots, a, o, st);
+  return sort_pass_t<TL, FIRST, LAST, 16, 4>(in, in_slots, a, o, st);
 }
 
 template <typename TL>
@@ -444,7 +450,7 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
       a.keys[i] = buf[2 * i];
       a.slots[i] = buf[2 * i + 1];
     }
-    e = n <= 1024 ? sort_block<TL, 1>(labels, a, o, st) : sort_block<TL, kBlockItems>(labels, a, o, st);
+    e = sort_block(labels, a, o, st);
   } else {
     SortPass a{};
     a.n = n;
@@ -455,23 +461,23 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
     a.total = reinterpret_cast<uint32_t*>(ws + al(static_cast<size_t>(p.bins) * p.tiles * 4));
     if (p.passes == 1) {
       a.mask = 0xffffffffu;
-      return sort_pass<TL, true, true>(labels, nullptr, a, o, st);
+      return sort_pass<TL, true, true>(p, labels, nullptr, a, o, st);
     }
     a.mask = static_cast<uint32_t>(p.bins - 1);
     o.keys = buf[0];
     o.slots = buf[1];
-    e = sort_pass<TL, true, false>(labels, nullptr, a, o, st);
+    e = sort_pass<TL, true, false>(p, labels, nullptr, a, o, st);
     const uint32_t *keys = buf[0], *slots = buf[1];
     if (e == cudaSuccess && p.passes == 3) {
       a.shift = p.bits;
       o.keys = buf[2];
       o.slots = buf[3];
-      e = sort_pass<uint32_t, false, false>(keys, slots, a, o, st);
+      e = sort_pass<uint32_t, false, false>(p, keys, slots, a, o, st);
       keys = buf[2];
       slots = buf[3];
     }
     a.shift = p.bits * (p.passes - 1);
-    if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(keys, slots, a, o, st);
+    if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(p, keys, slots, a, o, st);
   }
   if (e == cudaSuccess && p.passes > 1)
     e = launch_after(true, sort_offsets_kernel, static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st, sorted, n, k, offsets);

@@ -95,7 +95,7 @@ def test_groups_abi_checks(lib):
     # keep a histogram per tile too
     assert lib.euc_group_rows_workspace_bytes(1000, 64) == 0
     assert lib.euc_group_rows_workspace_bytes(1000, 100000) >= 2 * 4000
-    assert lib.euc_group_rows_workspace_bytes(1 << 20, 64) >= 65 * 512 * 4
+    assert lib.euc_group_rows_workspace_bytes(1 << 20, 64) >= 65 * 256 * 4
     f = lib.euc_group_rows
     assert f(P, 1, -1, 4, P, P, P, P, P, 1 << 20, None) == 1 and f(P, 1, 4, -1, P, P, P, P, P, 1 << 20, None) == 1
     assert f(P, 1, big, 4, P, P, P, P, P, 1 << 20, None) == 1 and f(P, 1, 4, big, P, P, P, P, P, 1 << 20, None) == 1
