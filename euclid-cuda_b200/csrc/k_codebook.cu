@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ C, in
     const WideRows<R, U> w(chunks);
     int64_t c[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) c[r] = w.row + r < n ? static_cast<int64_t>(labels[w.row + r]) : -1;
+    for (int r = 0; r < R; ++r) c[r] = w.row + r < n ? static_cast<int64_t>(__ldg(labels + w.row + r)) : -1;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ C, in
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w.at(u, row[u], v[u]);
-      c[u] = row[u] < n ? static_cast<int64_t>(labels[row[u]]) : -1;
+      c[u] = row[u] < n ? static_cast<int64_t>(__ldg(labels + row[u])) : -1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) lookup_any_kernel(const T* __restrict__ C
   for (int u = 0; u < 2; ++u) {
     uint32_t v;
     w.at(u, row[u], v);
-    c[u] = row[u] < n ? static_cast<int64_t>(labels[row[u]]) : -1;
+    c[u] = row[u] < n ? static_cast<int64_t>(__ldg(labels + row[u])) : -1;
     at[u] = static_cast<int>(v) * N -
             static_cast<int>((reinterpret_cast<uintptr_t>(out + row[u] * dim) & 15u) / sizeof(T));
     if (row[u] >= n) at[u] = dim;
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
 #pragma unroll
     for (int u = 0; u < RB; ++u) {
       const int64_t q = pb + u;
-      const int64_t row = q < p1 ? a.order[q] : -1;
-      lab[u] = q < p1 ? a.labels[q] : -1;
+      const int64_t row = q < p1 ? __ldg(a.order + q) : -1;
+      lab[u] = q < p1 ? __ldg(a.labels + q) : -1;
       g[u].raw = row >= 0 && row < a.n ? load_once(Gr + row * a.nv + v) : raw_zero<Raw>();
     }
 #pragma unroll
@@ -266,7 +266,7 @@ __device__ __forceinline__ void add_parts(const A* part, int64_t c, int64_t c1, 
       const int64_t q = c + u * step;
       const A* at = part + ((2 * q + (lo < q * seg ? 0 : 1)) * nv + v) * N;
 #pragma unroll
-      for (int e = 0; e < N; ++e) from[u][e] = q <= c1 ? at[e] : A(0);
+      for (int e = 0; e < N; ++e) from[u][e] = q <= c1 ? __ldcg(at + e) : A(0);
     }
 #pragma unroll
     for (int u = 0; u < P; ++u)

@@ -104,7 +104,6 @@ template <typename TL>
 __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__ in, BlockSort a, SortOut o) {
   extern __shared__ uint32_t sm[];
   __shared__ uint32_t warp_sums[32];
-  let_next_start();
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* start = sm;  // [bins] first position of the digit
   unsigned short* cnt = reinterpret_cast<unsigned short*>(sm + a.bins);  // [warps][bins]
@@ -169,7 +168,7 @@ struct SortPass {
 
 template <typename TL, bool FIRST> __device__ __forceinline__ uint32_t load_key(const TL* in, int64_t s, uint32_t k) {
   if constexpr (FIRST) return key_of(in[s], k);
-  else return static_cast<uint32_t>(in[s]);
+  else return static_cast<uint32_t>(__ldcg(in + s));
 }
 
 template <typename TL, bool FIRST, int WARPS, int ITEMS>
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(256) sort_tiles_kernel(SortPass a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int b = b0 + u * 32 + lane;
-      v[u] = b < quads ? row[b] : make_uint4(0u, 0u, 0u, 0u);
+      v[u] = b < quads ? __ldcg(row + b) : make_uint4(0u, 0u, 0u, 0u);
       x[u] = v[u].x + v[u].y + v[u].z + v[u].w;
     }
 #pragma unroll
@@ -280,13 +279,13 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
   __syncthreads();
   block_scan(local, a.bins, warp_sums);
   if (FIRST) wait_for_previous();
-  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) start[c] = a.total[c];
+  for (int c = threadIdx.x; c < a.bins; c += blockDim.x) start[c] = __ldcg(a.total + c);
   __syncthreads();
   block_scan(start, a.bins, warp_sums);
   if (LAST && o.offsets && blockIdx.x == 0)
     for (int c = threadIdx.x; c < a.bins; c += blockDim.x) o.offsets[c] = static_cast<int32_t>(start[c]);
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x)  // (every thread its own bins, as above)
-    start[c] += a.T[static_cast<int64_t>(c) * a.tiles + blockIdx.x] - local[c];
+    start[c] += __ldcg(a.T + static_cast<int64_t>(c) * a.tiles + blockIdx.x) - local[c];
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < ITEMS; ++u)
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
     const int64_t s = tile + (w & 0xffffu);
     const uint32_t pos = start[d] + l;
     const uint32_t key = FIRST && LAST ? d : load_key<TL, FIRST>(in, s, a.k);
-    const uint32_t slot = FIRST ? static_cast<uint32_t>(s) : in_slots[s];
+    const uint32_t slot = FIRST ? static_cast<uint32_t>(s) : __ldcg(in_slots + s);
     if (LAST) {
       const bool kept = key < a.k;
       o.order[pos] = kept ? static_cast<int32_t>(slot) : -1;
@@ -319,13 +318,13 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
 // offsets of a sort of several passes: first position whose key is not below c
 __global__ void sort_offsets_kernel(const int32_t* __restrict__ labels, int64_t n, int64_t k,
                                     int32_t* __restrict__ offsets) {
-  wait_for_previous();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (c > k) return;
   int64_t lo = 0, hi = n;  // dropped slots (-1, at the end) count as k
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    const int64_t v = labels[mid] < 0 ? k : labels[mid];
+    const int32_t l = __ldg(labels + mid);
+    const int64_t v = l < 0 ? k : l;
     if (v < c) lo = mid + 1; else hi = mid;
   }
   offsets[c] = static_cast<int32_t>(lo);
@@ -479,8 +478,10 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
     a.shift = p.bits * (p.passes - 1);
     if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(p, keys, slots, a, o, st);
   }
-  if (e == cudaSuccess && p.passes > 1)
-    e = launch_after(true, sort_offsets_kernel, static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st, sorted, n, k, offsets);
+  if (e == cudaSuccess && p.passes > 1) {  // (not early: its searches share L1)
+    sort_offsets_kernel<<<static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st>>>(sorted, n, k, offsets);
+    e = cudaGetLastError();
+  }
   return e;
 }
 
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(256) rows_to_groups_kernel(const R* __restrict
     for (int u = 0; u < U; ++u)
       if (w.v + 32 * u < nv) x[u] = load_once(X + w.row * nv + w.v + 32 * u);
     for (int j = 0; j < p; ++j) {
-      const int64_t r = position[w.row * p + j];
+      const int64_t r = __ldg(position + w.row * p + j);
       if (r < 0 || r >= slots) continue;
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(256) rows_to_groups_kernel(const R* __restrict
     for (int j = 0; j < p; ++j)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t r = row[u] < n ? position[row[u] * p + j] : -1;
+        const int64_t r = row[u] < n ? __ldg(position + row[u] * p + j) : -1;
         if (r >= 0 && r < slots) store_once(Y + r * nv + v[u], x[u]);
       }
   }
@@ -584,9 +585,9 @@ __global__ void __launch_bounds__(256) rows_from_groups_kernel(const T* __restri
     bool ok[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int64_t r = j0 + j < p ? pos[j0 + j] : -1;
+      const int64_t r = j0 + j < p ? __ldg(pos + j0 + j) : -1;
       ok[j] = r >= 0 && r < slots;
-      wt[j] = WEIGHTED && j0 + j < p ? wts[j0 + j] : A(1);
+      wt[j] = WEIGHTED && j0 + j < p ? __ldg(wts + j0 + j) : A(1);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         z[j][u].raw = raw_zero<Raw>();
@@ -651,11 +652,11 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         dot[j] = A(0);
-        r[j] = i < n && j0 + j < p ? position[i * p + j0 + j] : -1;
+        r[j] = i < n && j0 + j < p ? __ldg(position + i * p + j0 + j) : -1;
         if (r[j] >= slots) r[j] = -1;
       }
 #pragma unroll
-      for (int j = 0; j < J; ++j) wt[j] = weights && i < n && j0 + j < p ? weights[i * p + j0 + j] : A(1);
+      for (int j = 0; j < J; ++j) wt[j] = weights && i < n && j0 + j < p ? __ldg(weights + i * p + j0 + j) : A(1);
       for (int64_t v0 = in_team; v0 < nv && i < n; v0 += UV * TEAM) {
         V g[UV], z[UV][J];
 #pragma unroll

@@ -101,7 +101,8 @@ inline int row_vec_bytes(int64_t row_bytes, uintptr_t addresses) {
 
 // Programmatic dependent launch: a kernel launched with `early` may start while the one before
 // it on the stream still runs; what it does before wait_for_previous() reads nothing
-// that kernel writes and writes nothing that it touches.
+// that kernel writes and writes nothing that it touches, and what that kernel writes is read
+// behind it through L2 (ld.cg), past lines that an SM may hold from before.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
