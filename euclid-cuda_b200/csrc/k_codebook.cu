@@ -12,7 +12,10 @@
 // vector of the row) adds the chunk's rows in order; a label that lies inside the chunk is
 // rounded and written at once, one that crosses a chunk's border leaves its sum in the
 // workspace (slot 0 of the chunk if it began before the chunk, else slot 1), and a second
-// kernel adds those in chunk order and clears the rows of labels without rows.
+// kernel adds those in a fixed order.  The rows of labels without rows are cleared beside the
+// sums.  Bound by HBM where rows are many (1048576 of 128 fp32 to 1024: 100 us, 5.4 TB/s;
+// 65536 of 1024 bf16 to 131072, the frequent ones' rows in 60 chunks: 91, 4.4), and by the
+// latency of the join where they are few.
 #include "engine.h"
 #include "rows.cuh"
 

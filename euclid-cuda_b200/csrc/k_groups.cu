@@ -10,16 +10,21 @@
 //   dZ[position[i, j]] = w[i, j] dOut[i]  dw[i, j] = <dOut[i], Z[position[i, j]]>
 // and dX[i] = sum_j dY[position[i, j]], the second with weights of one.
 //
-// The sort is a counting sort in passes of up to kMaxBins bins (one pass where shared memory holds k + 1 bins,
-// else 2 or 3 by digits, least significant first); a slot is ranked among its warp's equal
-// keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit counters per warp
-// and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in 2.7 us.  More take
-// three kernels a pass (histograms of tiles, scan of each bin over the tiles, scatter through
-// shared memory so that a bin's run is stored together), 131072 slots of 128 labels in 6.7
-// us, 8192 of 256 in 7.1 (one block 23); one cluster of 8 blocks took 54 for them, since eight SMs scatter no faster.  The sort
-// moves 4 to 8 bytes a slot where the rows move kilobytes; the row kernels are bound by HBM,
-// and read and write every row once: a row's copies are written from registers after one
-// read, its weighted sum is formed from p reads.
+// The sort is a counting sort in passes of up to kMaxBins bins (one pass where shared memory
+// holds k + 1 bins, else 2 or 3 by digits, least significant first); a slot is ranked among
+// its warp's equal keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit
+// counters per warp and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in
+// 2.7 us.  More take three kernels a pass (histograms of tiles, scan of each bin over the
+// tiles, scatter through shared memory so that a bin's run is stored together): 131072 slots
+// of 128 labels in 6.7 us (one cluster of 8 blocks took 54: eight SMs scatter no faster),
+// 8192 of 256 in 7.1 (one block: 23).  The sort moves 4 to 8 bytes a slot where the rows move
+// kilobytes.
+//
+// The row kernels are bound by HBM, and read and write every row once: a row's copies are
+// written from registers after one read, its weighted sum is formed from p reads (16384 rows
+// of 2048 bf16, 8 picks: there 100 us at 6.0 TB/s, back 102 at 5.9, the way back's gradient
+// 201 at 5.7).  Rows that are not whole 16-byte words go by the widest part that divides them
+// (5003 rows of 1001 fp32, 3 picks, by 4 bytes: 15, 18 and 32 us, 4.3 to 5.2 TB/s).
 #include "engine.h"
 #include "rows.cuh"
 
@@ -28,11 +33,15 @@
 namespace euc {
 
 // ------------------------------------------------------------------ the sort
-constexpr int kBlockBins = 2049;  // k + 1 bins (the last for labels outside [0, k)) in one pass of a block,
-constexpr int kMaxBins = 4609;    // and of three kernels: what shared memory holds per warp and bin
-constexpr int kManyBins = 1537;   // of more than kManySlots slots (262144 of 3000 labels: 22 us in one pass, 27 in
-constexpr int64_t kManySlots = 1 << 18;  // two; 1048576 of 4000: 94 in one, 50 in two)
-constexpr int kPassBits = 11;     // digits of a sort of several passes, at most
+// k + 1 bins (the last for labels outside [0, k)) that one pass may have: of a block, and of
+// three kernels, what shared memory holds per warp and bin; of more than kManySlots slots,
+// what their histograms cost (262144 of 3000 labels: 22 us in one pass, 27 in two; 1048576 of
+// 4000: 94 in one, 50 in two).
+constexpr int kBlockBins = 2049;
+constexpr int kMaxBins = 4609;
+constexpr int kManyBins = 1537;
+constexpr int64_t kManySlots = 1 << 18;
+constexpr int kPassBits = 11;  // digits of a sort of several passes, at most
 
 struct SortOut {
   uint32_t* keys;  // a pass that is not the last: keys and slots in the pass's order
@@ -405,8 +414,8 @@ static cudaError_t sort_pass_t(const TL* in, const uint32_t* in_slots, const Sor
   if (e != cudaSuccess) return e;
   const unsigned tiles = static_cast<unsigned>((a.n + TILE - 1) / TILE);
   // Each kernel may start while the one before it runs, if all their blocks fit beside one
-  // another with little shared memory: 131072 slots of 128 labels take 8.1 us so, and 11.4
-  // one after another; but 1048576 slots of 1024 labels 40 us, and 33 one after another.
+  // another with little shared memory: 131072 slots of 128 labels took 8.1 us so (in tiles of
+  // 2048) and 11.4 one after another, but 1048576 slots of 1024 labels 40 us and 33.
   const bool early = a.bins <= 512 && static_cast<int>(tiles) <= num_sms();
   e = launch_after(!FIRST && early, hist, tiles, WARPS * 32, static_cast<size_t>(a.bins) * 4, st, in, a);
   if (e == cudaSuccess)
