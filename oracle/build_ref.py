@@ -77,7 +77,7 @@ def main():
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
-    if not os.path.isdir(a.src):
+    if not all(os.path.isfile(os.path.join(a.src, f)) for fs in EXTENSIONS.values() for f in fs):
         print(f"[build_ref] reference sources not found at {a.src}; skipping")
         return 0
     os.makedirs(OUT, exist_ok=True)
