@@ -126,6 +126,8 @@ int euc_group_rows(const void* labels, int labels_are_i64, int64_t slots, int64_
   const size_t need = group_ws_bytes(slots, k);
   if (need > 0 && (!ws || ws_bytes < need))
     return set_error(EUC_ERR_WORKSPACE, ("group_rows: workspace of " + std::to_string(need) + " bytes required").c_str());
+  if (need > 0 && reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+    return set_error(EUC_ERR_ARG, "group_rows: the workspace must start on a 16-byte boundary");
   return done(launch_group_rows(labels, labels_are_i64 != 0, slots, k, offsets, order, position, sorted_labels, ws,
                                 static_cast<cudaStream_t>(stream)),
               "group_rows");

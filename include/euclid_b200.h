@@ -369,7 +369,8 @@ EUC_API int euc_label_log_probs_grad(int row_type, const void* scores, int64_t l
  *   order[r]     slot at sorted position r, -1 for r >= offsets[k]
  *   position[s]  sorted position of slot s, -1 if dropped
  *   sorted_labels[r]  label at sorted position r, -1 for r >= offsets[k]
- * slots and k are at most 2^31 - 2; dim, in all of these, at most 2^30. */
+ * slots and k are at most 2^31 - 2; dim, in all of these, at most 2^30.  `ws` starts on a
+ * 16-byte boundary. */
 EUC_API size_t euc_group_rows_workspace_bytes(int64_t slots, int64_t k);
 EUC_API int euc_group_rows(const void* labels, int labels_are_i64, int64_t slots, int64_t k, int32_t* offsets,
                    int32_t* order, int32_t* position, int32_t* sorted_labels, void* ws, size_t ws_bytes,

@@ -108,6 +108,7 @@ def test_groups_abi_checks(lib):
         assert b(0, P, P, P, 4, 2, 8, P, None) == 8 and g(0, P, P, P, P, P, 4, 2, 8, P, P, None) == 8
     else:
         assert f(P, 1, 4, 10000, P, P, P, P, P, 16, None) == 6      # EUC_ERR_WORKSPACE
+        assert f(P, 1, 4, 10000, P, P, P, P, ctypes.c_void_p(264), 1 << 20, None) == 7  # workspace off 16 bytes
         assert f(P, 1, 4, 4, P, None, P, P, P, 1 << 20, None) == 7
         assert t(0, None, P, P, 4, 2, 8, P, None) == 7 and b(0, P, P, P, 4, 2, 8, None, None) == 7
         assert t(0, ctypes.c_void_p(258), P, P, 4, 2, 8, P, None) == 7
