@@ -246,6 +246,36 @@ def test_autograd_in_the_scores_type_and_broadcast_gradients():
     assert torch.equal(x.grad, label_log_probs_grad(x.detach(), lab, r.row_stats, None, one, 1.5))
 
 
+def test_autograd_without_labels_or_rows():
+    x, _ = make(4, 50, torch.float32, seed=6)
+    x = x.clone().requires_grad_()
+    r = label_log_probs(x, None, 0.5, 2)
+    assert r.log_probs is None
+    r.entropy.sum().backward()
+    one = torch.ones(4, device="cuda")
+    assert torch.equal(x.grad, label_log_probs_grad(x.detach(), None, r.row_stats, None, one, 0.5))
+    e = torch.empty(0, 50, device="cuda", requires_grad=True)
+    label_log_probs(e, torch.empty(0, dtype=torch.int64, device="cuda")).log_probs.sum().backward()
+    assert e.grad.shape == (0, 50)
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams, interleaved, with inputs of their own."""
+    jobs = []
+    for s in range(2):
+        x, lab = make(300, 20000, torch.bfloat16, seed=40 + s)
+        jobs.append((torch.cuda.Stream(), x, lab, label_log_probs(x, lab, 1.0, 8), []))
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for st, x, lab, _, got in jobs:
+            with torch.cuda.stream(st):
+                got.append(label_log_probs(x, lab, 1.0, 8))
+    torch.cuda.synchronize()
+    for _, _, _, want, got in jobs:
+        for r in got:
+            assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 @pytest.mark.parametrize("n,m", [(1, 131072), (300, 1000), (3, 40000)])
 def test_same_result_every_time_and_any_place(n, m):
     """A row's outputs do not depend on the run, nor on the other rows."""

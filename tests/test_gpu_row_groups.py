@@ -222,6 +222,34 @@ def test_other_stream_captured_and_repeated():
         assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_no_picks():
+    g = group_rows(torch.empty(5, 0, dtype=torch.int64, device="cuda"), 3)
+    assert g.picks == 0 and g.n_rows == 5 and g.offsets.tolist() == [0] * 4
+    X = torch.randn(5, 8, device="cuda")
+    Y = rows_to_groups(X, g)
+    assert Y.shape == (0, 8) and torch.equal(rows_from_groups(Y, g), torch.zeros_like(X))
+    gY, gW = rows_from_groups_grad(X, Y, g, torch.empty(5, 0, device="cuda"))
+    assert gY.shape == (0, 8) and gW.shape == (5, 0)
+
+
+@pytest.mark.parametrize("n,k", [(100000, 100), (100000, 3000), (60000, 70000)])
+def test_two_streams_at_once(n, k):
+    """Sorts whose kernels overlap, on two streams at once and one behind the other."""
+    jobs = []
+    for s in range(2):
+        lab = make_labels((n,), k, 50 + s, "skew")
+        jobs.append((torch.cuda.Stream(), lab, group_rows(lab, k), []))
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for st, lab, _, got in jobs:
+            with torch.cuda.stream(st):
+                got.append(group_rows(lab, k))
+    torch.cuda.synchronize()
+    for _, _, want, got in jobs:
+        for r in got:
+            assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_refusals():
     lab = make_labels((10, 2), 4, 1)
     g = group_rows(lab, 4)
