@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
       const uint32_t l = local[digit[u]] + mine[digit[u]] + rank[u];
       stage[l] = (digit[u] << 16) | static_cast<uint32_t>(first + u * 32);
       // of a sort of one pass the digit is the key, and neighbouring lanes have neighbouring slots
-      if (FIRST && LAST) o.position[tile + first + u * 32] = digit[u] < a.k ? static_cast<int32_t>(start[digit[u]] + l) : -1;
+      if (FIRST && LAST)
+        o.position[tile + first + u * 32] = digit[u] < a.k ? static_cast<int32_t>(start[digit[u]] + l) : -1;
     }
   __syncthreads();
   const int here = static_cast<int>(min(static_cast<int64_t>((WARPS * 32 * ITEMS)), a.n - tile));
@@ -387,17 +388,19 @@ size_t group_ws_bytes(int64_t n, int64_t k) {
 }
 
 // dynamic shared memory beyond the 48 KiB that a launch may ask for unannounced, of which the
-// kernels' static arrays take a little
-static cudaError_t more_smem(const void* kernel, size_t bytes) {
+// kernels' static arrays take a little; always the most that the kernel takes, so that calls
+// of different sizes from several threads do not lower one another's limit
+static cudaError_t more_smem(const void* kernel, size_t bytes, int most) {
   if (bytes <= 47 * 1024) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
 }
 
 template <typename TL>
 static cudaError_t sort_block(const TL* in, const BlockSort& a, const SortOut& o, cudaStream_t st) {
   const int nt = (a.n + 31) / 32 * 32;
   const size_t smem = static_cast<size_t>(a.bins) * (4 + 2 * (nt / 32));
-  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_block_kernel<TL>), smem);
+  constexpr int kMost = std::max(kBlockBins, 1 << kPassBits) * (4 + 2 * static_cast<int>(kBlockSlots / 32));
+  const cudaError_t e = more_smem(reinterpret_cast<const void*>(sort_block_kernel<TL>), smem, kMost);
   if (e != cudaSuccess) return e;
   sort_block_kernel<TL><<<1, nt, smem, st>>>(in, a, o);
   return cudaGetLastError();
@@ -407,10 +410,11 @@ template <typename TL, bool FIRST, bool LAST, int WARPS, int ITEMS>
 static cudaError_t sort_pass_t(const TL* in, const uint32_t* in_slots, const SortPass& a, const SortOut& o,
                                cudaStream_t st) {
   constexpr int TILE = WARPS * 32 * ITEMS;
+  constexpr int kMost = std::max(kMaxBins, 1 << kPassBits) * (8 + 2 * WARPS) + TILE * 4;
   const auto hist = sort_hist_kernel<TL, FIRST, WARPS, ITEMS>;
   const auto scatter = sort_scatter_kernel<TL, FIRST, LAST, WARPS, ITEMS>;
   const size_t sm = static_cast<size_t>(a.bins) * (8 + 2 * WARPS) + TILE * 4;
-  cudaError_t e = more_smem(reinterpret_cast<const void*>(scatter), sm);
+  cudaError_t e = more_smem(reinterpret_cast<const void*>(scatter), sm, kMost);
   if (e != cudaSuccess) return e;
   const unsigned tiles = static_cast<unsigned>((a.n + TILE - 1) / TILE);
   // Each kernel may start while the one before it runs, if all their blocks fit beside one

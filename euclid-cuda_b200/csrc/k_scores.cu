@@ -389,7 +389,7 @@ template <typename A> __device__ __forceinline__ int place_of(const Key<A>* list
 }
 
 // ------------------------------------------------------------------ a team of lanes per row
-// Rows of up to TEAM EPL scores, a team of 8 or 32 lanes each: the row stays in registers, so
+// Rows of up to TEAM EPL scores, a team of 8, 16 or 32 lanes each: the row stays in registers, so
 // its scores are read once and its maximum is known before the first exponential; a warp
 // reads its next rows while it works on these, into shared memory, which leaves the registers
 // to more warps (131072 x 1024 fp32 with the 8 best: 156 us with the next row in registers
@@ -604,7 +604,8 @@ template <typename A> struct Part {  // one block's share of a row
 };
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1) scores_block_kernel(ScoreArgs<T> a, int log_cluster, int per_group) {
+__global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1)
+    scores_block_kernel(ScoreArgs<T> a, int log_cluster, int per_group) {
   using A = Acc<T>;
   constexpr int VE = RowVecs<T>::VE, U = kBlockVecs, W = NT / 32, LISTS = W == 1 ? U : 1;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -629,7 +630,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1) scores_blo
   // the first and the last vector where they are not whole: the first and the last thread
   int edge = -1;
   if (threadIdx.x == 0 && row.lo > 0 && v0 == 0) edge = 0;
-  if (threadIdx.x == NT - 1 && row.hi < row.all && v1 == row.all && v0 < v1 && !(row.lo > 0 && row.all == 1)) edge = row.all - 1;
+  if (threadIdx.x == NT - 1 && row.hi < row.all && v1 == row.all && v0 < v1 && !(row.lo > 0 && row.all == 1))
+    edge = row.all - 1;
   if (threadIdx.x == 0) count_sh = hits_sh = 0;
   __syncwarp();
   if (cluster > 1) cluster_arrive();  // waited for before the first store to another block
