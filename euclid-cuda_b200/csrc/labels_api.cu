@@ -35,10 +35,18 @@ static int rows_shape(int64_t n, int64_t p, int64_t dim) {
   return EUC_OK;
 }
 
-static bool misaligned(int t, std::initializer_list<const void*> ps) {
+using Pointers = std::initializer_list<const void*>;
+
+// whether a pointer is off its elements: rows of the row type, fp32 or fp64 values, int32
+// indexes, labels of either type
+static bool off(size_t bytes, Pointers ps) {
   for (const void* p : ps)
-    if (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(type_size(t))) return true;
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return true;
   return false;
+}
+static bool misaligned(int t, Pointers rows, Pointers values, Pointers indexes, const void* labels, bool labels_i64) {
+  return off(type_size(t), rows) || off(t == EUC_ROW_F64 ? 8 : 4, values) || off(4, indexes) ||
+         off(labels_i64 ? 8 : 4, {labels});
 }
 
 static int scores_shape(int row_type, int64_t ld, int64_t n, int64_t m, double scale) {
@@ -67,7 +75,9 @@ int euc_label_log_probs(int row_type, const void* scores, int64_t ld, int64_t n,
   if (n == 0) return EUC_OK;
   if (!scores || (log_probs && !labels) || (top > 0 && (!top_log_probs || !top_labels)))
     return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {scores})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {scores}, {log_probs, entropy, row_stats, top_log_probs}, {}, labels, labels_are_i64 != 0) ||
+      off(8, {top_labels}))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   ScoreJob j{};
   j.x = scores;
   j.ld = ld;
@@ -94,7 +104,8 @@ int euc_label_log_probs_grad(int row_type, const void* scores, int64_t ld, int64
   if (int rc = no_device()) return rc;
   if (n == 0) return EUC_OK;
   if (!scores || !row_stats || !grad || (grad_log_probs && !labels)) return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {scores, grad})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {scores, grad}, {row_stats, grad_log_probs, grad_entropy}, {}, labels, labels_are_i64 != 0))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   ScoreGradJob j{};
   j.x = scores;
   j.ld = ld;
@@ -123,10 +134,13 @@ int euc_group_rows(const void* labels, int labels_are_i64, int64_t slots, int64_
   if (int rc = no_device()) return rc;
   if (!offsets || (slots > 0 && (!labels || !order || !position || !sorted_labels)))
     return set_error(EUC_ERR_ARG, "null pointer");
+  if (misaligned(EUC_ROW_F32, {}, {}, {offsets, order, position, sorted_labels}, labels, labels_are_i64 != 0))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   const size_t need = group_ws_bytes(slots, k);
   if (need > 0 && (!ws || ws_bytes < need))
-    return set_error(EUC_ERR_WORKSPACE, ("group_rows: workspace of " + std::to_string(need) + " bytes required").c_str());
-  if (need > 0 && reinterpret_cast<uintptr_t>(ws) % 16 != 0)
+    return set_error(EUC_ERR_WORKSPACE,
+                     ("group_rows: workspace of " + std::to_string(need) + " bytes required").c_str());
+  if (need > 0 && off(16, {ws}))
     return set_error(EUC_ERR_ARG, "group_rows: the workspace must start on a 16-byte boundary");
   return done(launch_group_rows(labels, labels_are_i64 != 0, slots, k, offsets, order, position, sorted_labels, ws,
                                 static_cast<cudaStream_t>(stream)),
@@ -140,7 +154,8 @@ int euc_rows_to_groups(int row_type, const void* X, const int32_t* position, con
   if (int rc = no_device()) return rc;
   if (n == 0 || p == 0 || dim == 0) return EUC_OK;
   if (!X || !position || !kept || !Y) return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {X, Y})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {X, Y}, {}, {position, kept}, nullptr, false))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   return done(launch_rows_to_groups(type_size(row_type), X, position, kept, n, static_cast<int>(p), dim, Y,
                                     static_cast<cudaStream_t>(stream)),
               "rows_to_groups");
@@ -153,7 +168,8 @@ int euc_rows_from_groups(int row_type, const void* Y, const int32_t* position, c
   if (int rc = no_device()) return rc;
   if (n == 0 || dim == 0) return EUC_OK;
   if (!out || (p > 0 && (!Y || !position))) return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {Y, out})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {Y, out}, {weights}, {position}, nullptr, false))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   return done(launch_rows_from_groups(static_cast<RowType>(row_type), Y, position, weights, n, static_cast<int>(p), dim,
                                       out, static_cast<cudaStream_t>(stream)),
               "rows_from_groups");
@@ -168,7 +184,8 @@ int euc_rows_from_groups_grad(int row_type, const void* grad_out, const void* Y,
   if (n == 0 || p == 0) return EUC_OK;
   if (!position || !kept || (dim > 0 && (!grad_out || !grad_Y || (grad_weights && !Y))))
     return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {grad_out, Y, grad_Y})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {grad_out, Y, grad_Y}, {weights, grad_weights}, {position, kept}, nullptr, false))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   if (dim == 0) {  // empty products
     if (!grad_weights) return EUC_OK;
     return done(cudaMemsetAsync(grad_weights, 0, static_cast<size_t>(n) * p * (row_type == EUC_ROW_F64 ? 8 : 4),
@@ -189,7 +206,8 @@ int euc_codebook_lookup(int row_type, const void* C, int64_t k, const void* labe
   if (int rc = no_device()) return rc;
   if (n == 0 || dim == 0) return EUC_OK;
   if (!labels || !out || (k > 0 && !C)) return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {C, out})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {C, out}, {}, {}, labels, labels_are_i64 != 0))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   return done(launch_codebook_lookup(static_cast<RowType>(row_type), C, k, labels, labels_are_i64 != 0, n, dim, scale,
                                      out, static_cast<cudaStream_t>(stream)),
               "codebook_lookup");
@@ -210,10 +228,12 @@ int euc_codebook_grad(int row_type, const void* grad_out, const int32_t* offsets
   if (k == 0 || dim == 0) return EUC_OK;
   if (!offsets || !grad_C || (n > 0 && (!grad_out || !order || !sorted_labels)))
     return set_error(EUC_ERR_ARG, "null pointer");
-  if (misaligned(row_type, {grad_out, grad_C})) return set_error(EUC_ERR_ARG, "misaligned pointer");
+  if (misaligned(row_type, {grad_out, grad_C}, {ws}, {offsets, order, sorted_labels}, nullptr, false))
+    return set_error(EUC_ERR_ARG, "misaligned pointer");
   const size_t need = euc_codebook_grad_workspace_bytes(row_type, n, dim);
   if (need > 0 && (!ws || ws_bytes < need))
-    return set_error(EUC_ERR_WORKSPACE, ("codebook_grad: workspace of " + std::to_string(need) + " bytes required").c_str());
+    return set_error(EUC_ERR_WORKSPACE,
+                     ("codebook_grad: workspace of " + std::to_string(need) + " bytes required").c_str());
   return done(launch_codebook_grad(static_cast<RowType>(row_type), grad_out, offsets, order, sorted_labels, n, k, dim,
                                    scale, grad_C, ws, static_cast<cudaStream_t>(stream)),
               "codebook_grad");

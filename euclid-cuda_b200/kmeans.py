@@ -105,6 +105,8 @@ class LloydKMeans:
         if not temperature > 0:
             raise RuntimeError("temperature must be positive")
         n, m = X.size(0), C.size(0)
+        if labels is not None and tuple(labels.shape) != (n,):
+            raise RuntimeError(f"labels must have shape {(n,)}")
         rows = int(block_rows) if block_rows else max(1, (1 << 30) // max(1, m * X.element_size()))
         parts = []
         for lo in range(0, n, rows) if n > 0 else (0,):

@@ -338,7 +338,8 @@ EUC_API int euc_kmeanspp(const void* X, int x_is_f64, int64_t n, int64_t dim, in
  * No counterpart in the reference.  What a caller does with labels: how sure a label
  * is, rows brought together by label and back, and codebook rows from labels; each
  * with its gradient.  All results are the same on every run (no atomics on values).
- * Sums, weights and statistics are fp32, and fp64 for fp64 rows. */
+ * Sums, weights and statistics are fp32, and fp64 for fp64 rows.  Every pointer is aligned
+ * to its elements (a workspace of sums to the sums'). */
 typedef enum { EUC_ROW_F32 = 0, EUC_ROW_F64 = 1, EUC_ROW_F16 = 2, EUC_ROW_BF16 = 3 } euc_row_type;
 
 /* Log probabilities of n rows of m <= 2^30 scores (row stride ld >= m elements), z = scale * x:

@@ -52,6 +52,8 @@ def test_cpu_tensors_are_refused():
         row_groups.rows_to_groups(x, (lab,))
     with pytest.raises(RuntimeError, match="temperature"):
         kmeans.LloydKMeans(3).posterior(x, x, temperature=0.0)
+    with pytest.raises(RuntimeError, match="labels must have shape"):
+        kmeans.LloydKMeans(3).posterior(x, x, labels=torch.zeros(5, dtype=torch.int64))
 
 
 @pytest.fixture(scope="module")
@@ -79,12 +81,16 @@ def test_scores_abi_checks(lib):
     else:  # refused before any launch
         assert call(x=None) == 7 and call(lab=None, lp=P) == 7 and call(top=1) == 7
         assert call(x=ctypes.c_void_p(258)) == 7 and call(n=0) == 0
+        off4, off2 = ctypes.c_void_p(260), ctypes.c_void_p(258)
+        assert call(lab=off4, lp=P) == 7 and call(lp=off2) == 7 and call(top=1, tlp=P, tl=off4) == 7
     g = lib.euc_label_log_probs_grad
     assert g(0, P, 8, 4, 8, P, 1, 0.0, P, P, None, P, None) == 7
     assert g(0, P, 7, 4, 8, P, 1, 1.0, P, P, None, P, None) == 1
     if not NO_GPU:
         assert g(0, P, 8, 4, 8, None, 1, 1.0, P, P, None, P, None) == 7
         assert g(0, P, 8, 4, 8, P, 1, 1.0, None, P, None, P, None) == 7
+        assert g(0, P, 8, 4, 8, P, 1, 1.0, off2, P, None, P, None) == 7
+        assert g(1, P, 8, 4, 8, P, 1, 1.0, P, off4, None, P, None) == 7
 
 
 def test_groups_abi_checks(lib):
@@ -113,6 +119,10 @@ def test_groups_abi_checks(lib):
         assert t(0, None, P, P, 4, 2, 8, P, None) == 7 and b(0, P, P, P, 4, 2, 8, None, None) == 7
         assert t(0, ctypes.c_void_p(258), P, P, 4, 2, 8, P, None) == 7
         assert g(0, P, None, P, P, P, 4, 2, 8, P, P, None) == 7
+        off = ctypes.c_void_p(258)
+        assert f(P, 1, 4, 4, P, off, P, P, P, 1 << 20, None) == 7 and f(off, 0, 4, 4, P, P, P, P, P, 0, None) == 7
+        assert t(2, P, off, P, 4, 2, 8, P, None) == 7 and b(2, P, P, off, 4, 2, 8, P, None) == 7
+        assert g(2, P, P, P, P, P, 4, 2, 8, P, off, None) == 7
 
 
 def test_codebook_abi_checks(lib):
@@ -128,3 +138,7 @@ def test_codebook_abi_checks(lib):
     else:
         assert f(0, None, 4, P, 1, 4, 8, 1.0, P, None) == 7
         assert g(0, P, P, P, P, 4, 4, 8, 1.0, P, P, 16, None) == 6
+        off = ctypes.c_void_p(258)
+        assert f(2, P, 4, off, 0, 4, 8, 1.0, P, None) == 7
+        assert g(2, P, P, P, P, 4, 4, 8, 1.0, P, off, 1 << 20, None) == 7
+        assert g(2, P, P, off, P, 4, 4, 8, 1.0, P, P, 1 << 20, None) == 7
