@@ -137,27 +137,28 @@ def rows_from_groups_grad(grad_out, Y, groups, weights=None):
 class _ToGroups(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X, groups):
-        ctx.groups = groups
-        return _to_groups(X, groups)
+        Y = _to_groups(X, groups)
+        ctx.save_for_backward(*groups)  # (refuses a backward pass after a change in place)
+        return Y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        return _from_groups(g.contiguous(), ctx.groups, None), None
+        return _from_groups(g.contiguous(), RowGroups(*ctx.saved_tensors), None), None
 
 
 class _FromGroups(torch.autograd.Function):
     @staticmethod
     def forward(ctx, Y, groups, weights):
-        ctx.groups = groups
-        ctx.save_for_backward(Y, weights)
-        return _from_groups(Y, groups, weights)
+        out = _from_groups(Y, groups, weights)
+        ctx.save_for_backward(Y, weights, *groups)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        Y, weights = ctx.saved_tensors
-        grad_Y, grad_w = rows_from_groups_grad(g.contiguous(), Y, ctx.groups, weights)
+        Y, weights, *groups = ctx.saved_tensors
+        grad_Y, grad_w = rows_from_groups_grad(g.contiguous(), Y, RowGroups(*groups), weights)
         return grad_Y, None, grad_w
 
 

@@ -1,5 +1,7 @@
 """group_rows, rows_to_groups, rows_from_groups and the gradients against their definitions:
 the stable order exactly, the rows there exactly, the sums within their derived bounds."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -248,6 +250,42 @@ def test_two_streams_at_once(n, k):
     for _, _, want, got in jobs:
         for r in got:
             assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
+@pytest.mark.parametrize("n", [1000, 4000])
+def test_threads_with_sizes_of_their_own(n):
+    """One kernel with little and with much shared memory, from two threads at once."""
+    wrong = []
+
+    def sort(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            lab = make_labels((n,), k, 60, "uniform")
+            want = group_rows(lab, k)
+            for _ in range(200):
+                try:
+                    got = group_rows(lab, k)
+                except RuntimeError as e:
+                    wrong.append(f"{k}: {e}")
+                    return
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                wrong.append(f"{k}: other groups")
+
+    threads = [threading.Thread(target=sort, args=(k,)) for k in (1500, 1900, 2040, 1700)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_groups_changed_before_the_backward_pass():
+    g = group_rows(make_labels((20, 2), 4, 1), 4)
+    X = torch.randn(20, 8, device="cuda", requires_grad=True)
+    out = rows_from_groups(rows_to_groups(X, g), g)
+    g.position.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
 
 
 def test_refusals():
