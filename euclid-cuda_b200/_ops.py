@@ -235,7 +235,7 @@ def check_like(t, name, shape, dtype, device):
     check_input(t, name)
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {_DT_NAME[dtype]}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:  # (torch.Size, or a tuple)
         raise RuntimeError(f"{name} must have shape {tuple(shape)}")
     if t.device != device:
         raise RuntimeError(f"{name} must be on {device}")

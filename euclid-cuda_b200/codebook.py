@@ -21,7 +21,7 @@ def _lookup(C, labels, scale):
     i64 = _ops.check_labels(labels)
     _ops.check_same_device(labels, "labels", C, "C")
     k, d = C.shape
-    out = torch.empty((*labels.shape, d), dtype=C.dtype, device=C.device)
+    out = C.new_empty((*labels.shape, d))
     call_on(C, lib().euc_codebook_lookup, rt, C.data_ptr(), k, labels.data_ptr(), i64, labels.numel(), d, scale,
             out.data_ptr())
     return out
@@ -41,12 +41,12 @@ def lookup_grad(G, labels, n_clusters, scale=1.0, groups=None):
     if groups is None:
         groups = group_rows(labels.reshape(-1), k)
     else:
-        check_groups(groups)
-        if groups.n_clusters != k or groups.order.numel() != n:
+        rows, picks, clusters = check_groups(groups)
+        if clusters != k or rows * picks != n:
             raise RuntimeError("groups do not belong to these labels")
         _ops.check_same_device(groups.order, "groups", G, "G")
     d = G.size(-1)
-    out = torch.empty((k, d), dtype=G.dtype, device=G.device)
+    out = G.new_empty((k, d))
     ws = workspace(lib().euc_codebook_grad_workspace_bytes(rt, n, d), G.device)
     call_on(G, lib().euc_codebook_grad, rt, G.data_ptr(), groups.offsets.data_ptr(), groups.order.data_ptr(),
             groups.labels.data_ptr(), n, k, d, float(scale), out.data_ptr(), ws.data_ptr(), ws.numel())

@@ -56,12 +56,12 @@ def _forward(scores, labels, scale, top):
     n, m, ld, rt, i64 = _check(scores, labels, scale)
     if not 0 <= top <= min(m, MAX_TOP):
         raise RuntimeError(f"top must be in [0, min(columns, {MAX_TOP})]")
-    dev, acc = scores.device, _ops.acc_dtype(scores)
-    log_probs = torch.empty(n, dtype=acc, device=dev) if labels is not None else None
-    entropy = torch.empty(n, dtype=acc, device=dev)
-    stats = torch.empty((n, 3), dtype=acc, device=dev)
-    top_lp = torch.empty((n, top), dtype=acc, device=dev)
-    top_lab = torch.empty((n, top), dtype=torch.int64, device=dev)
+    new, acc = scores.new_empty, _ops.acc_dtype(scores)  # (2 us less a call than torch.empty)
+    log_probs = new(n, dtype=acc) if labels is not None else None
+    entropy = new(n, dtype=acc)
+    stats = new((n, 3), dtype=acc)
+    top_lp = new((n, top), dtype=acc)
+    top_lab = new((n, top), dtype=torch.int64)
     call_on(scores, lib().euc_label_log_probs, rt, scores.data_ptr(), ld, n, m,
             labels.data_ptr() if labels is not None else None, i64, scale, top,
             log_probs.data_ptr() if labels is not None else None, entropy.data_ptr(), stats.data_ptr(),
@@ -116,7 +116,7 @@ def label_log_probs_grad(scores, labels, row_stats, grad_log_probs=None, grad_en
         _ops.check_like(grad_log_probs, "grad_log_probs", (n,), acc, scores.device)
     if grad_entropy is not None:
         _ops.check_like(grad_entropy, "grad_entropy", (n,), acc, scores.device)
-    grad = torch.empty((n, m), dtype=scores.dtype, device=scores.device)
+    grad = scores.new_empty((n, m))
     call_on(scores, lib().euc_label_log_probs_grad, rt, scores.data_ptr(), ld, n, m,
             labels.data_ptr() if labels is not None else None, i64, scale, row_stats.data_ptr(),
             grad_log_probs.data_ptr() if grad_log_probs is not None else None,

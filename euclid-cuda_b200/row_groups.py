@@ -49,22 +49,23 @@ def group_rows(labels, n_clusters):
     i64 = _ops.check_labels(labels)
     if labels.dim() not in (1, 2):
         raise RuntimeError("labels must be 1D or 2D")
-    k, slots, dev = int(n_clusters), labels.numel(), labels.device
+    k, slots, new = int(n_clusters), labels.numel(), labels.new_empty
     if k < 0 or k > 2 ** 31 - 2 or slots > 2 ** 31 - 2:
         raise RuntimeError("n_clusters and the number of labels must be in [0, 2^31 - 2]")
-    offsets = torch.empty(k + 1, dtype=torch.int32, device=dev)
-    order = torch.empty(slots, dtype=torch.int32, device=dev)
-    position = torch.empty(labels.shape, dtype=torch.int32, device=dev)
-    sorted_labels = torch.empty(slots, dtype=torch.int32, device=dev)
+    offsets = new(k + 1, dtype=torch.int32)
+    order = new(slots, dtype=torch.int32)
+    position = new(labels.shape, dtype=torch.int32)
+    sorted_labels = new(slots, dtype=torch.int32)
     need = lib().euc_group_rows_workspace_bytes(slots, k)
-    ws = workspace(need, dev) if need else None
+    ws = workspace(need, labels.device) if need else None
     call_on(labels, lib().euc_group_rows, labels.data_ptr(), i64, slots, k, offsets.data_ptr(), order.data_ptr(),
             position.data_ptr(), sorted_labels.data_ptr(), ws.data_ptr() if need else None, need)
     return RowGroups(offsets, order, position, sorted_labels)
 
 
 def check_groups(groups):
-    """A RowGroups whose parts fit together (their values are checked by the kernels)."""
+    """A RowGroups whose parts fit together (their values are checked by the kernels):
+    (rows, picks, clusters)."""
     if not isinstance(groups, RowGroups):
         raise TypeError("groups must be a RowGroups")
     offsets, order, position, labels = groups
@@ -72,10 +73,11 @@ def check_groups(groups):
         _ops.check_input(t, name)
         if t.dtype != torch.int32 or t.get_device() != offsets.get_device():
             raise RuntimeError(f"groups.{name} must be int32 on the groups' device")
-    slots = position.numel()
-    if offsets.dim() != 1 or offsets.numel() < 1 or position.dim() not in (1, 2) or \
+    slots, shape = position.numel(), position.shape
+    if offsets.dim() != 1 or offsets.numel() < 1 or len(shape) not in (1, 2) or \
             order.numel() != slots or labels.numel() != slots:
         raise RuntimeError("groups do not fit together")
+    return shape[0], shape[1] if len(shape) == 2 else 1, offsets.numel() - 1
 
 
 def _check_rows(t, name, rows, groups):
@@ -84,19 +86,18 @@ def _check_rows(t, name, rows, groups):
     if t.dim() != 2 or t.size(0) != rows:
         raise RuntimeError(f"{name} must be 2D with {rows} rows")
     _ops.check_same_device(t, name, groups.position, "groups")
-    return rt
+    return rt, t.size(1)
 
 
-def _kept(groups):
-    return groups.offsets.data_ptr() + 4 * groups.n_clusters
+def _kept(groups, k):
+    return groups.offsets.data_ptr() + 4 * k
 
 
 def _to_groups(X, groups):
-    check_groups(groups)
-    n, p = groups.n_rows, groups.picks
-    rt = _check_rows(X, "X", n, groups)
-    Y = torch.empty((n * p, X.size(1)), dtype=X.dtype, device=X.device)
-    call_on(X, lib().euc_rows_to_groups, rt, X.data_ptr(), groups.position.data_ptr(), _kept(groups), n, p, X.size(1),
+    n, p, k = check_groups(groups)
+    rt, d = _check_rows(X, "X", n, groups)
+    Y = X.new_empty((n * p, d))
+    call_on(X, lib().euc_rows_to_groups, rt, X.data_ptr(), groups.position.data_ptr(), _kept(groups, k), n, p, d,
             Y.data_ptr())
     return Y
 
@@ -107,13 +108,12 @@ def _check_weights(weights, Y, groups):
 
 
 def _from_groups(Y, groups, weights):
-    check_groups(groups)
-    n, p = groups.n_rows, groups.picks
-    rt = _check_rows(Y, "Y", n * p, groups)
+    n, p, _ = check_groups(groups)
+    rt, d = _check_rows(Y, "Y", n * p, groups)
     _check_weights(weights, Y, groups)
-    out = torch.empty((n, Y.size(1)), dtype=Y.dtype, device=Y.device)
+    out = Y.new_empty((n, d))
     call_on(Y, lib().euc_rows_from_groups, rt, Y.data_ptr(), groups.position.data_ptr(),
-            weights.data_ptr() if weights is not None else None, n, p, Y.size(1), out.data_ptr())
+            weights.data_ptr() if weights is not None else None, n, p, d, out.data_ptr())
     return out
 
 
@@ -121,15 +121,14 @@ def rows_from_groups_grad(grad_out, Y, groups, weights=None):
     """Gradients of rows_from_groups: (grad_Y, grad_weights), the second None without
     weights.  grad_Y[position[i, j]] = weights[i, j] * grad_out[i], zero rows behind the
     last kept slot; grad_weights[i, j] = <grad_out[i], Y[position[i, j]]>, 0 where dropped."""
-    check_groups(groups)
-    n, p = groups.n_rows, groups.picks
-    rt = _check_rows(Y, "Y", n * p, groups)
+    n, p, k = check_groups(groups)
+    rt, d = _check_rows(Y, "Y", n * p, groups)
     _check_weights(weights, Y, groups)
-    _ops.check_like(grad_out, "grad_out", (n, Y.size(1)), Y.dtype, Y.device)
+    _ops.check_like(grad_out, "grad_out", (n, d), Y.dtype, Y.device)
     grad_Y = torch.empty_like(Y)
     grad_w = torch.empty_like(weights) if weights is not None else None
     call_on(Y, lib().euc_rows_from_groups_grad, rt, grad_out.data_ptr(), Y.data_ptr(), groups.position.data_ptr(),
-            weights.data_ptr() if weights is not None else None, _kept(groups), n, p, Y.size(1), grad_Y.data_ptr(),
+            weights.data_ptr() if weights is not None else None, _kept(groups, k), n, p, d, grad_Y.data_ptr(),
             grad_w.data_ptr() if weights is not None else None)
     return grad_Y, grad_w
 
