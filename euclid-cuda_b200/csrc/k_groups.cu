@@ -35,8 +35,9 @@ namespace euc {
 // ------------------------------------------------------------------ the sort
 // k + 1 bins (the last for labels outside [0, k)) that one pass may have: of a block, and of
 // three kernels, what shared memory holds per warp and bin; of more than kManySlots slots,
-// what their histograms cost (262144 of 3000 labels: 22 us in one pass, 27 in two; 1048576 of
-// 4000: 94 in one, 50 in two).
+// what their histograms cost (262144 of 2900 labels: 22 us in one pass, 27 in two; 1048576 of
+// 4000: 94 in one, 50 in two).  30011 of 4099 take 25 us in one pass and 18.6 in two, but
+// the four launches more cost the host 5 us more than that.
 constexpr int kBlockBins = 2049;
 constexpr int kMaxBins = 4609;
 constexpr int kManyBins = 1537;
@@ -325,17 +326,31 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
   }
 }
 
-// offsets of a sort of several passes: first position whose key is not below c
-__global__ void sort_offsets_kernel(const int32_t* __restrict__ labels, int64_t n, int64_t k,
+// offsets of a sort of several passes: first position whose key is not below c, between two
+// of kSamples evenly spaced positions, whose keys the block holds
+constexpr int kSamples = 256;
+
+__global__ void sort_offsets_kernel(const int32_t* __restrict__ labels, int64_t n, int k,
                                     int32_t* __restrict__ offsets) {
+  __shared__ int32_t sample[kSamples];
+  wait_for_previous();
+  auto key = [&](int64_t at) {  // dropped slots (-1, at the end) count as k
+    const int32_t l = __ldcg(labels + at);
+    return l < 0 ? k : l;
+  };
+  const int64_t step = (n + kSamples - 1) / kSamples;
+  for (int i = threadIdx.x; i < kSamples; i += blockDim.x) sample[i] = i * step < n ? key(i * step) : k;
+  __syncthreads();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (c > k) return;
-  int64_t lo = 0, hi = n;  // dropped slots (-1, at the end) count as k
+  int below = 0;  // samples below c
+  for (int half = kSamples / 2; half > 0; half /= 2)
+    if (sample[below + half - 1] < c) below += half;
+  below += sample[below] < c;
+  int64_t lo = below > 0 ? (below - 1) * step + 1 : 0, hi = min(n, below * step);
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    const int32_t l = __ldg(labels + mid);
-    const int64_t v = l < 0 ? k : l;
-    if (v < c) lo = mid + 1; else hi = mid;
+    if (key(mid) < c) lo = mid + 1; else hi = mid;
   }
   offsets[c] = static_cast<int32_t>(lo);
 }
@@ -418,9 +433,14 @@ static cudaError_t sort_pass_t(const TL* in, const uint32_t* in_slots, const Sor
   if (e != cudaSuccess) return e;
   const unsigned tiles = static_cast<unsigned>((a.n + TILE - 1) / TILE);
   // Each kernel may start while the one before it runs, if all their blocks fit beside one
-  // another with little shared memory: 131072 slots of 128 labels took 8.1 us so (in tiles of
-  // 2048) and 11.4 one after another, but 1048576 slots of 1024 labels 40 us and 33.
-  const bool early = a.bins <= 512 && static_cast<int>(tiles) <= num_sms();
+  // another with little shared memory and few counts to pass on: 131072 slots of 128 labels
+  // took 8.1 us so (in tiles of 2048) and 11.4 one after another, 16384 of 700 8.8 and 11.3,
+  // but 30011 of 1000 23 and 14; in two passes, 40000 of 131072 23.1 and 26.0, but 131072 of
+  // 131072 34 and 28.
+  const int64_t counts = static_cast<int64_t>(a.bins) * tiles;
+  const bool fits = FIRST && LAST ? a.bins <= 512 || (a.bins <= 1025 && counts <= 21000)
+                                  : a.bins <= 512 && tiles <= 64;
+  const bool early = fits && static_cast<int>(tiles) <= num_sms();
   e = launch_after(!FIRST && early, hist, tiles, WARPS * 32, static_cast<size_t>(a.bins) * 4, st, in, a);
   if (e == cudaSuccess)
     e = launch_after(early, sort_tiles_kernel, static_cast<unsigned>((a.bins + 7) / 8), 256, 0, st, a);
@@ -491,10 +511,9 @@ static cudaError_t group_t(const TL* labels, int64_t n, int64_t k, int32_t* offs
     a.shift = p.bits * (p.passes - 1);
     if (e == cudaSuccess) e = sort_pass<uint32_t, false, true>(p, keys, slots, a, o, st);
   }
-  if (e == cudaSuccess && p.passes > 1) {  // (not early: its searches share L1)
-    sort_offsets_kernel<<<static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st>>>(sorted, n, k, offsets);
-    e = cudaGetLastError();
-  }
+  if (e == cudaSuccess && p.passes > 1)
+    e = launch_after(true, sort_offsets_kernel, static_cast<unsigned>((k + 1 + 255) / 256), 256, 0, st, sorted, n,
+                     static_cast<int>(k), offsets);
   return e;
 }
 
