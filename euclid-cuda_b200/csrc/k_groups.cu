@@ -12,7 +12,7 @@
 //
 // The sort is a counting sort in passes of up to kMaxBins bins (one pass where shared memory
 // holds k + 1 bins, else 2 or 3 by digits, least significant first); a slot is ranked among
-// its warp's equal keys by __match_any_sync, 32 slots at a time in slot order, with 16-bit
+// its warp's equal keys by ballots, 32 slots at a time in slot order, with 16-bit
 // counters per warp and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in
 // 2.7 us.  More take three kernels a pass (histograms of tiles, scan of each bin over the
 // tiles, scatter through shared memory so that a bin's run is stored together): 131072 slots
@@ -82,23 +82,38 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int m, uint32_t* warp_su
   __syncthreads();
 }
 
-// rank[u] <- slots of the warp before (u, lane) with its digit; counts <- slots per digit
+// rank[u] <- slots of the warp before (u, lane) with its digit; counts <- slots per digit.
+// The lanes with a lane's digit come from a ballot per bit: match_any, whose lanes take turns,
+// costs more from a few labels up (1048576 slots of 4, 64 and 1024: 12.6, 18.4 and 26.7 us with
+// it, 13.4, 14.9 and 23.2 so).
 template <int ITEMS>
 __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], unsigned short (&rank)[ITEMS],
-                                           unsigned short* counts, int lane) {
+                                           unsigned short* counts, int lane, int bits) {
+  unsigned peers[ITEMS];
+#pragma unroll
+  for (int u = 0; u < ITEMS; ++u) peers[u] = __ballot_sync(0xffffffffu, digit[u] != 0xffffffffu);
+  for (int b = 0; b < bits; ++b)
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const bool one = digit[u] >> b & 1u;
+      const unsigned ones = __ballot_sync(0xffffffffu, one);
+      peers[u] &= one ? ones : ~ones;
+    }
 #pragma unroll
   for (int u = 0; u < ITEMS; ++u) {
     const bool in = digit[u] != 0xffffffffu;
-    const unsigned peers = __match_any_sync(0xffffffffu, digit[u]);
-    const int before = __popc(peers & ((1u << lane) - 1u));
+    const int before = __popc(peers[u] & ((1u << lane) - 1u));
     unsigned short base = 0;
     if (in) base = counts[digit[u]];
     __syncwarp();
-    if (in && before == 0) counts[digit[u]] = static_cast<unsigned short>(base + __popc(peers));
+    if (in && before == 0) counts[digit[u]] = static_cast<unsigned short>(base + __popc(peers[u]));
     rank[u] = static_cast<unsigned short>(base + before);
     __syncwarp();
   }
 }
+
+// bits of the digits below `bins`
+__device__ __forceinline__ int digit_bits(int bins) { return 32 - __clz(bins - 1); }
 
 // ---- all passes in one block
 struct BlockSort {
@@ -130,7 +145,7 @@ __global__ void __launch_bounds__(1024) sort_block_kernel(const TL* __restrict__
     unsigned short rank[1];
     for (int c = threadIdx.x; c < a.bins * warps; c += blockDim.x) cnt[c] = 0;
     __syncthreads();
-    warp_ranks<1>(digit, rank, mine, lane);
+    warp_ranks<1>(digit, rank, mine, lane, digit_bits(a.bins));
     __syncthreads();
     for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
       uint32_t run = 0;
@@ -274,7 +289,7 @@ __global__ void __launch_bounds__(WARPS * 32) sort_scatter_kernel(const TL* __re
     digit[u] = s < a.n ? (load_key<TL, FIRST>(in, s, a.k) >> a.shift) & a.mask : 0xffffffffu;
   }
   __syncthreads();
-  warp_ranks<ITEMS>(digit, rank, mine, lane);
+  warp_ranks<ITEMS>(digit, rank, mine, lane, digit_bits(a.bins));
   __syncthreads();
   for (int c = threadIdx.x; c < a.bins; c += blockDim.x) {  // counts -> prefixes over the warps
     uint32_t run = 0;
@@ -364,11 +379,14 @@ struct SortPlan {
 };
 
 // Tiles: small ones fill the SMs, and are cheap to begin while the bins are few; large ones
-// leave fewer histograms to add up (131072 slots of 128 labels: 6.7, 8.3 and 11.0 us with
-// 8 x 4, 16 x 4 and 16 x 8; 65536 of 1024: 13.9, 14.9, 18.2; 1048576 of 1024: 41, 35, 27).
+// leave fewer histograms to add up (131072 slots of 128 labels: 6.3, 7.5 and 9.5 us with
+// 8 x 4, 16 x 4 and 16 x 8; 65536 of 1024: 13.3, 14.1, 19.2; 1048576 of 1024: 36, 32, 25).
+// Where only 16 x 4 are at most one per SM, their kernels overlap (200000 of 128: 9.5, 7.5, 9.5).
+constexpr int64_t kSmsOfB200 = 148;
+
 static void set_tiles(SortPlan& p, int64_t n) {
-  const bool many = n > (1 << 19);
-  p.warps = !many && p.bins <= 1025 ? 8 : 16;
+  const bool many = n > (1 << 19), one_each = n > kSmsOfB200 * 1024 && n <= kSmsOfB200 * 2048;
+  p.warps = !many && !one_each && p.bins <= 1025 ? 8 : 16;
   p.items = many ? 8 : 4;
   const int tile = p.warps * 32 * p.items;
   p.tiles = static_cast<int>(((n + tile - 1) / tile + 3) / 4 * 4);
