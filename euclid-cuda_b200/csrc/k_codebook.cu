@@ -167,6 +167,23 @@ __device__ __forceinline__ void clear_rows(const GradArgs& a, int64_t block, int
   }
 }
 
+// Blocks that clear and blocks that sum take turns, so that one's writes and the other's
+// reads overlap.
+struct Role {
+  int64_t block;  // among the blocks of its kind
+  bool clears;
+  __device__ __forceinline__ Role(int64_t chunk_blocks) : block(blockIdx.x) {
+    const int64_t clear_blocks = gridDim.x - chunk_blocks, both = 2 * min(chunk_blocks, clear_blocks);
+    clears = chunk_blocks < clear_blocks;
+    if (block < both) {
+      clears = block & 1;
+      block >>= 1;
+    } else {
+      block -= both / 2;
+    }
+  }
+};
+
 template <typename T, int N>
 __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3 : 4)
     grad_chunks_kernel(const T* __restrict__ G, GradArgs a, int64_t chunk_blocks, Acc<T> scale, T* __restrict__ out,
@@ -177,23 +194,13 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
   const Raw* Gr = reinterpret_cast<const Raw*>(G);
   Raw* Or = reinterpret_cast<Raw*>(out);
   let_next_start();
-  // blocks that clear and blocks that sum take turns, so that one's writes and the other's
-  // reads overlap
-  const int64_t clear_blocks = gridDim.x - chunk_blocks, both = 2 * min(chunk_blocks, clear_blocks);
-  int64_t block = blockIdx.x;
-  bool clears = chunk_blocks < clear_blocks;
-  if (block < both) {
-    clears = block & 1;
-    block >>= 1;
-  } else {
-    block -= both / 2;
-  }
-  if (clears) {
-    clear_rows<Raw>(a, block, clear_blocks, Or);
+  const Role role(chunk_blocks);
+  if (role.clears) {
+    clear_rows<Raw>(a, role.block, gridDim.x - chunk_blocks, Or);
     return;
   }
   const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
-  const int64_t t = block * blockDim.x + threadIdx.x;
+  const int64_t t = role.block * blockDim.x + threadIdx.x;
   const int64_t chunk = t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(a.nv) : t / a.nv;
   const int64_t v = t - chunk * a.nv;
   const int64_t p0 = chunk * a.seg;
@@ -243,6 +250,99 @@ __global__ void __launch_bounds__(256, N * sizeof(T) == 16 && sizeof(T) == 2 ? 3
       }
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] += to_acc(g[u].e[e]);
+    }
+  }
+  flush();
+}
+
+// The same for 16-bit rows of odd length (a.nv of them): a thread adds the 16 bytes of the row
+// from element 8 v on, shifted out of the two aligned words that hold them, and leaves its
+// sums by elements, as the kernel above does with N = 1 (33588 rows of 999 bf16 to 30 and 1000
+// labels: 75 and 96 us element by element, 46 and 66 so; rows that 4 bytes divide are no
+// faster so).
+template <typename T>
+__global__ void __launch_bounds__(256, 3)
+    grad_chunks_any_kernel(const T* __restrict__ G, GradArgs a, int vecs, int64_t chunk_blocks, Acc<T> scale,
+                           T* __restrict__ out, Acc<T>* __restrict__ part) {
+  using A = Acc<T>;
+  constexpr int N = 8;
+  let_next_start();
+  const Role role(chunk_blocks);
+  if (role.clears) {
+    clear_rows(a, role.block, gridDim.x - chunk_blocks, reinterpret_cast<unsigned short*>(out));
+    return;
+  }
+  const int64_t total = min(a.n, static_cast<int64_t>(a.offsets[a.k]));
+  const int64_t t = role.block * blockDim.x + threadIdx.x;
+  const int64_t chunk = t < 0x80000000ll ? static_cast<uint32_t>(t) / static_cast<uint32_t>(vecs) : t / vecs;
+  const int64_t p0 = chunk * a.seg;
+  if (p0 >= total) return;
+  const int64_t p1 = min(total, p0 + a.seg);
+  const int64_t at = (t - chunk * vecs) * N;
+  const int count = static_cast<int>(min(static_cast<int64_t>(N), a.nv - at));  // elements of the row
+  const void *begin = G, *end = G + a.n * a.nv;
+  A acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = A(0);
+  int c = a.labels[p0];
+  bool from_left = p0 > 0 && a.labels[p0 - 1] == c;
+  const int behind = p1 < total ? a.labels[p1] : -1;
+  auto flush = [&]() {
+    if (c >= 0 && c < a.k) {
+      const bool whole = !from_left && c != behind;
+      T* o = out + c * a.nv + at;
+      A* to = part + (2 * chunk + (from_left ? 0 : 1)) * a.nv + at;
+      if (whole && count == N) {  // four 4-byte words, or three between two elements
+        Vec<T, N> x;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x.e[e] = from_acc<T>(scale * acc[e]);
+        const bool even = (reinterpret_cast<uintptr_t>(o) & 2u) == 0;
+        if (!even) {
+          o[0] = x.e[0];
+          o[N - 1] = x.e[N - 1];
+          x.raw = shift_16(x.raw, x.raw, 2u);
+        }
+        uint32_t* words = reinterpret_cast<uint32_t*>(o + (even ? 0 : 1));
+        store_once(words, x.raw.x);
+        store_once(words + 1, x.raw.y);
+        store_once(words + 2, x.raw.z);
+        if (even) store_once(words + 3, x.raw.w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (e < count) {
+            if (whole) o[e] = from_acc<T>(scale * acc[e]);
+            else to[e] = acc[e];
+          }
+      }
+    }
+    from_left = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = A(0);
+  };
+  constexpr int RB = 4;  // rows in flight
+  for (int64_t pb = p0; pb < p1; pb += RB) {
+    Words16 g[RB];
+    int32_t lab[RB];
+#pragma unroll
+    for (int u = 0; u < RB; ++u) {
+      const int64_t q = pb + u;
+      const int64_t row = q < p1 ? __ldg(a.order + q) : -1;
+      lab[u] = q < p1 ? __ldg(a.labels + q) : -1;
+      g[u].clear();
+      if (row >= 0 && row < a.n) g[u].load(G + row * a.nv + at, 0, count, begin, end);
+    }
+#pragma unroll
+    for (int u = 0; u < RB; ++u) {
+      if (pb + u >= p1) break;
+      if (lab[u] != c) {
+        flush();
+        c = lab[u];
+      }
+      Vec<T, N> x;
+      x.raw = g[u].get();
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += to_acc(x.e[e]);
     }
   }
   flush();
@@ -431,15 +531,24 @@ static cudaError_t lookup_n(const T* C, int64_t k, const void* labels, bool i64,
              : lookup_go<T, N>(C, k, static_cast<const int*>(labels), n, dim, scale, out, st);
 }
 
+// `vecs`: vectors of a row of odd length that is read 16 bytes at a time (N = 1), else 0
 template <typename T, int N>
-static cudaError_t grad_n(const T* G, GradArgs a, int64_t dim, double scale, T* out, void* ws, cudaStream_t st) {
+static cudaError_t grad_n(const T* G, GradArgs a, int64_t dim, int64_t vecs, double scale, T* out, void* ws,
+                          cudaStream_t st) {
   a.nv = dim / N;
   Acc<T>* part = static_cast<Acc<T>*>(ws);
   const Acc<T> s = static_cast<Acc<T>>(scale);
-  const int64_t sums = (a.chunks * a.nv + 255) / 256;
+  const int64_t sums = (a.chunks * (vecs ? vecs : a.nv) + 255) / 256;
   const int64_t clears = std::min<int64_t>(
       ((a.k + 31) / 32 * ((a.nv + kClearVecs - 1) / kClearVecs) + 7) / 8, static_cast<int64_t>(num_sms()) * 16);
-  grad_chunks_kernel<T, N><<<static_cast<unsigned>(sums + clears), 256, 0, st>>>(G, a, sums, s, out, part);
+  const unsigned blocks = static_cast<unsigned>(sums + clears);
+  bool any = false;
+  if constexpr (N == 1 && sizeof(T) == 2) {
+    any = vecs > 0;
+    if (any)
+      grad_chunks_any_kernel<T><<<blocks, 256, 0, st>>>(G, a, static_cast<int>(vecs), sums, s, out, part);
+  }
+  if (!any) grad_chunks_kernel<T, N><<<blocks, 256, 0, st>>>(G, a, sums, s, out, part);
   if (a.chunks > 1) {
     int width = 32;
     while (width > 1 && width / 2 >= a.nv) width /= 2;
@@ -488,7 +597,9 @@ static cudaError_t grad_t(const void* G, const GradArgs& a, int64_t dim, double 
                           cudaStream_t st) {
   const int b = row_vec_bytes(dim * static_cast<int64_t>(sizeof(T)),
                               reinterpret_cast<uintptr_t>(G) | reinterpret_cast<uintptr_t>(out));
-  EUC_ROW_VEC(T, b, grad_n, static_cast<const T*>(G), a, dim, scale, static_cast<T*>(out), ws, st);
+  if (b == 2 && dim >= 32)  // (a million rows of 5: 26 us by elements and 29 so)
+    return grad_n<T, 1>(static_cast<const T*>(G), a, dim, (dim + 7) / 8, scale, static_cast<T*>(out), ws, st);
+  EUC_ROW_VEC(T, b, grad_n, static_cast<const T*>(G), a, dim, 0, scale, static_cast<T*>(out), ws, st);
 }
 
 cudaError_t launch_codebook_lookup(RowType t, const void* C, int64_t k, const void* labels, bool labels_i64, int64_t n,

@@ -60,6 +60,21 @@ template <> struct BitsOf<2> { using type = unsigned short; };
 template <> struct BitsOf<4> { using type = uint32_t; };
 template <> struct BitsOf<8> { using type = unsigned long long; };
 
+// the 16 bytes that begin `shift` (even, below 16) bytes behind the start of (a, b)
+__device__ __forceinline__ uint4 shift_16(const uint4& a, const uint4& b, unsigned shift) {
+  const unsigned bits = (shift & 3u) * 8u;
+  auto pick = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4) {
+    return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                      __funnelshift_r(w3, w4, bits));
+  };
+  switch (shift >> 2) {  // the same for all vectors of a row
+    case 0: return pick(a.x, a.y, a.z, a.w, b.x);
+    case 1: return pick(a.y, a.z, a.w, b.x, b.y);
+    case 2: return pick(a.z, a.w, b.x, b.y, b.z);
+    default: return pick(a.w, b.x, b.y, b.z, b.w);
+  }
+}
+
 // The 16 bytes at any address that T's alignment allows, from the two aligned 16-byte words
 // that hold them (neighbouring lanes share them, so the second comes from L1); element by
 // element where one of the words is not inside [begin, end).
@@ -78,18 +93,49 @@ __device__ __forceinline__ uint4 load_any_16(const T* p, const void* begin, cons
     for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) v.e[e] = reinterpret_cast<const Bits*>(p)[e];
     return v.raw;
   }
-  const uint4 a = load_keep(w), b = load_keep(w + 1);
-  const unsigned bits = static_cast<unsigned>(shift & 3u) * 8u;
-  auto pick = [&](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t w4) {
-    return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
-                      __funnelshift_r(w3, w4, bits));
-  };
-  switch (shift >> 2) {  // the same for all vectors of a row
-    case 0: return pick(a.x, a.y, a.z, a.w, b.x);
-    case 1: return pick(a.y, a.z, a.w, b.x, b.y);
-    case 2: return pick(a.z, a.w, b.x, b.y, b.z);
-    default: return pick(a.w, b.x, b.y, b.z, b.w);
+  return shift_16(load_keep(w), load_keep(w + 1), static_cast<unsigned>(shift));
+}
+
+// The same for elements [first, last) of the 8 at `from` (16-bit ones, those around them not
+// looked at), as the two words and the shift, so that several such loads are in flight at once.
+struct Words16 {
+  uint4 lo, hi;
+  unsigned shift;
+  __device__ __forceinline__ void clear() {
+    lo = hi = make_uint4(0u, 0u, 0u, 0u);
+    shift = 0u;
   }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* from, int first, int last, const void* begin, const void* end) {
+    static_assert(sizeof(T) == 2, "16-bit elements");
+    shift = static_cast<unsigned>(reinterpret_cast<uintptr_t>(from) & 15u);
+    const uint4* w = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(from) - shift);
+    if (static_cast<const void*>(w) >= begin && static_cast<const void*>(w + 2) <= end) {
+      lo = load_keep(w);
+      hi = load_keep(w + 1);
+      return;
+    }
+    Vec<T, 8> x;  // at the buffer's ends: element by element
+    x.raw = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e >= first && e < last) x.e[e] = from[e];
+    lo = x.raw;
+    hi = make_uint4(0u, 0u, 0u, 0u);
+    shift = 0u;
+  }
+  __device__ __forceinline__ uint4 get() const { return shift_16(lo, hi, shift); }
+};
+
+// 8 16-bit elements to a 16-byte boundary, but for those outside [first, last)
+template <typename T> __device__ __forceinline__ void store_16(T* to, const Vec<T, 8>& x, int first, int last) {
+  if (first <= 0 && last >= 8) {
+    store_once(reinterpret_cast<uint4*>(to), x.raw);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e >= first && e < last) to[e] = x.e[e];
 }
 
 // Bytes of the widest vector that every row of `row_bytes` starts and ends on, given the

@@ -82,6 +82,23 @@ def test_long_labels(n, k, d, kind):
     check(C, G, make_labels((n,), k, n, kind), 0.5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,k,d,kind", [(20000, 50, 45, "skew"), (3000, 1500, 333, "drop"), (1, 1, 33, "even"),
+                                        (17, 2, 39, "one"), (4000, 3, 2049, "even"), (5000, 9000, 77, "skew")])
+def test_odd_rows_of_16_bits(n, k, d, kind, dtype):
+    g = gen(n + d)
+    C = torch.randn(k, d, generator=g, device="cuda", dtype=torch.float64).to(dtype)
+    G = torch.randn(n, d, generator=g, device="cuda", dtype=torch.float64).to(dtype)
+    lab = make_labels((n,), k, n, kind)
+    got = check(C, G, lab, 0.75)
+    # (neighbouring rows share 16-byte words: a NaN stays in its own label's row)
+    G[n // 2] = float("nan")
+    bad = lookup_grad(G, lab, k, 0.75).isnan()
+    l = int(lab[n // 2])
+    assert int(bad.sum()) == (d if 0 <= l < k else 0)
+    assert not got.isnan().any() and (not 0 <= l < k or bad[l].all())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shift", [1, 2, 4])
 def test_alignments_and_shapes(dtype, shift):

@@ -224,6 +224,21 @@ def test_other_stream_captured_and_repeated():
         assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [33, 45, 333])
+def test_odd_rows_of_16_bits(d, dtype):
+    """Neighbouring rows share 16-byte words: what is in one reaches no other's sum."""
+    check_rows(700, 6, 20, d, dtype, "drop", d)
+    g = group_rows(make_labels((700, 3), 20, d, "even"), 20)
+    Y = torch.randn(2100, d, generator=gen(d), device="cuda").to(dtype)
+    bad = [0, 1, 999, 2099]
+    Y[bad] = float("nan")
+    out = rows_from_groups(Y, g).isnan()
+    want = torch.zeros(700, dtype=torch.bool, device="cuda")
+    want[(g.order[bad] // 3).long()] = True
+    assert torch.equal(out, want[:, None].expand(700, d))
+
+
 def test_no_picks():
     g = group_rows(torch.empty(5, 0, dtype=torch.int64, device="cuda"), 3)
     assert g.picks == 0 and g.n_rows == 5 and g.offsets.tolist() == [0] * 4
