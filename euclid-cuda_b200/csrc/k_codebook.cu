@@ -597,7 +597,9 @@ static cudaError_t grad_t(const void* G, const GradArgs& a, int64_t dim, double 
                           cudaStream_t st) {
   const int b = row_vec_bytes(dim * static_cast<int64_t>(sizeof(T)),
                               reinterpret_cast<uintptr_t>(G) | reinterpret_cast<uintptr_t>(out));
-  if (b == 2 && dim >= 32)  // (a million rows of 5: 26 us by elements and 29 so)
+  // (with fewer threads, latency counts: 30011 rows of 77 to 4099 labels 13.7 us by elements and
+  // 19 so, 94720 to 11840 35 and 31; a million rows of 5: 26 and 29)
+  if (b == 2 && dim >= 32 && a.chunks * ((dim + 7) / 8) >= static_cast<int64_t>(num_sms()) * 320)
     return grad_n<T, 1>(static_cast<const T*>(G), a, dim, (dim + 7) / 8, scale, static_cast<T*>(out), ws, st);
   EUC_ROW_VEC(T, b, grad_n, static_cast<const T*>(G), a, dim, 0, scale, static_cast<T*>(out), ws, st);
 }

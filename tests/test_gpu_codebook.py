@@ -84,7 +84,9 @@ def test_long_labels(n, k, d, kind):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("n,k,d,kind", [(20000, 50, 45, "skew"), (3000, 1500, 333, "drop"), (1, 1, 33, "even"),
-                                        (17, 2, 39, "one"), (4000, 3, 2049, "even"), (5000, 9000, 77, "skew")])
+                                        (17, 2, 39, "one"), (4000, 3, 2049, "even"), (5000, 9000, 77, "skew"),
+                                        (200000, 50, 45, "skew"), (30000, 1500, 333, "drop"), (160000, 2, 39, "one"),
+                                        (100000, 90000, 77, "even"), (150000, 7, 33, "drop")])
 def test_odd_rows_of_16_bits(n, k, d, kind, dtype):
     g = gen(n + d)
     C = torch.randn(k, d, generator=g, device="cuda", dtype=torch.float64).to(dtype)

@@ -225,18 +225,18 @@ def test_other_stream_captured_and_repeated():
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("d", [33, 45, 333])
-def test_odd_rows_of_16_bits(d, dtype):
+@pytest.mark.parametrize("n,d", [(700, 33), (700, 45), (700, 333), (12000, 33), (9000, 47), (1500, 333), (30, 16001)])
+def test_odd_rows_of_16_bits(n, d, dtype):
     """Neighbouring rows share 16-byte words: what is in one reaches no other's sum."""
-    check_rows(700, 6, 20, d, dtype, "drop", d)
-    g = group_rows(make_labels((700, 3), 20, d, "even"), 20)
-    Y = torch.randn(2100, d, generator=gen(d), device="cuda").to(dtype)
-    bad = [0, 1, 999, 2099]
+    check_rows(n, 6, 20, d, dtype, "drop", d)
+    g = group_rows(make_labels((n, 3), 20, d, "even"), 20)
+    Y = torch.randn(3 * n, d, generator=gen(d), device="cuda").to(dtype)
+    bad = [0, 1, n, 3 * n - 1]
     Y[bad] = float("nan")
     out = rows_from_groups(Y, g).isnan()
-    want = torch.zeros(700, dtype=torch.bool, device="cuda")
+    want = torch.zeros(n, dtype=torch.bool, device="cuda")
     want[(g.order[bad] // 3).long()] = True
-    assert torch.equal(out, want[:, None].expand(700, d))
+    assert torch.equal(out, want[:, None].expand(n, d))
 
 
 def test_no_picks():
