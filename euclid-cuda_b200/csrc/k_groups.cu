@@ -14,10 +14,10 @@
 // holds k + 1 bins, else 2 or 3 by digits, least significant first); a slot is ranked among
 // its warp's equal keys by ballots, 32 slots at a time in slot order, with 16-bit
 // counters per warp and bin.  Up to kBlockSlots slots one block runs all passes, 64 slots in
-// 2.7 us.  More take three kernels a pass (histograms of tiles, scan of each bin over the
+// 2.8 us.  More take three kernels a pass (histograms of tiles, scan of each bin over the
 // tiles, scatter through shared memory so that a bin's run is stored together): 131072 slots
-// of 128 labels in 6.7 us (one cluster of 8 blocks took 54: eight SMs scatter no faster),
-// 8192 of 256 in 7.1 (one block: 23).  The sort moves 4 to 8 bytes a slot where the rows move
+// of 128 labels in 6.3 us (one cluster of 8 blocks took 54: eight SMs scatter no faster),
+// 8192 of 256 in 6.8 (one block: 23).  The sort moves 4 to 8 bytes a slot where the rows move
 // kilobytes.
 //
 // The row kernels are bound by HBM, and read and write every row once: a row's copies are
