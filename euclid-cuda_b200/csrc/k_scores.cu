@@ -6,7 +6,8 @@
 //   log p_j = z_j - M - L        entropy H = L - T / S
 //   dz_j = g_l ([j = l] - p_j) - g_H p_j (log p_j + H),  dx_j = scale * dz_j
 // z_j - M is formed as (y_j - max y) |scale| with y = sign(scale) x, which loses nothing
-// to a common offset of the scores.  T and H are sums of terms of one sign.
+// to a common offset of the scores.  Where the difference is beyond the type, p_j is 0: the
+// smallest |scale| that is taken makes it so.  T and H are sums of terms of one sign.
 //
 // Masked scores (z = -inf) have probability 0 and add nothing.  A row with no score left
 // has log probabilities of -inf, entropy 0 and a zero gradient; a row that holds a NaN or
@@ -182,6 +183,16 @@ template <typename T> __device__ __forceinline__ int64_t label_of(const void* la
   return i64 ? static_cast<const long long*>(labels)[i] : static_cast<const int*>(labels)[i];
 }
 
+// (y - hi) mag - L of a row.  Above 1, hi may be so large that the difference is beyond the type
+// and its product with mag is not: half the difference is taken twice as often then, which
+// rounds as the whole one does.
+template <typename A> struct LogProb {
+  A part, hi, mag, L;
+  __device__ __forceinline__ LogProb(A hi_, A mag_, A L_)
+      : part(hi_ > A(1) ? A(0.5) : A(1)), hi(hi_ * part), mag(hi_ > A(1) ? mag_ * A(2) : mag_), L(L_) {}
+  __device__ __forceinline__ A operator()(A y) const { return fma(y, part, -hi) * mag - L; }
+};
+
 // the row's outputs from its M (as max y), S, T, L = log S (-inf for an empty row), and the
 // score at its label (`in`: the label is one of the columns)
 template <typename T>
@@ -196,7 +207,7 @@ __device__ __forceinline__ void write_row(const ScoreArgs<T>& a, int64_t i, Acc<
     a.stats[3 * i + 1] = L;
     a.stats[3 * i + 2] = H;
   }
-  if (a.log_probs) a.log_probs[i] = !in ? A(0) : empty ? neg_inf<A>() : (at_label - hi) * a.mag - L;
+  if (a.log_probs) a.log_probs[i] = !in ? A(0) : empty ? neg_inf<A>() : LogProb<A>(hi, a.mag, L)(at_label);
 }
 
 // ------------------------------------------------------------------ a row as vectors
@@ -381,7 +392,7 @@ template <typename T>
 __device__ __forceinline__ void write_top(const ScoreArgs<T>& a, int64_t i, int place, const Key<Acc<T>>& k, Acc<T> hi,
                                           Acc<T> L) {
   a.top_labels[i * a.top + place] = k.j();
-  a.top_log_probs[i * a.top + place] = hi == neg_inf<Acc<T>>() ? hi : (k.y() - hi) * a.mag - L;
+  a.top_log_probs[i * a.top + place] = hi == neg_inf<Acc<T>>() ? hi : LogProb<Acc<T>>(hi, a.mag, L)(k.y());
 }
 
 // how many of list[0, count) are ahead of `me`

@@ -53,9 +53,13 @@ static int scores_shape(int row_type, int64_t ld, int64_t n, int64_t m, double s
   if (n < 0 || n > kMaxIndex || m < 1 || m > kMaxScores) return set_error(EUC_ERR_SHAPE, "scores: bad size");
   if (ld < m && n > 1) return set_error(EUC_ERR_SHAPE, "scores: row stride below the row's length");
   if (!std::isfinite(scale) || scale == 0.0) return set_error(EUC_ERR_ARG, "scale must be finite and not 0");
-  // the fp32 arithmetic holds |scale| and its multiple of log2(e) as normal numbers
-  if (row_type != EUC_ROW_F64 && !(std::fabs(scale) >= 0x1p-126 && std::fabs(scale) <= 0x1p126))
-    return set_error(EUC_ERR_ARG, "scale is outside fp32's range");
+  // the arithmetic holds |scale|, twice it and its multiple of log2(e) as normal numbers; scores
+  // with the exponents of fp32 or fp64 may differ by more than their type holds, by 2^128 or
+  // 2^1024, and times |scale| that is 256 or 1024 at least: exp of minus that is 0
+  const double least = row_type == EUC_ROW_F64 ? 0x1p-1014 : row_type == EUC_ROW_F16 ? 0x1p-126 : 0x1p-120;
+  const double most = row_type == EUC_ROW_F64 ? 0x1p1022 : 0x1p126;
+  if (!(std::fabs(scale) >= least && std::fabs(scale) <= most))
+    return set_error(EUC_ERR_ARG, "scale is outside the range of the scores' type");
   return EUC_OK;
 }
 

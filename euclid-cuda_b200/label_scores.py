@@ -95,6 +95,7 @@ def label_log_probs(scores, labels=None, scale=1.0, top=0):
     labels (int64 or int32 [n], optional).  `top` (at most 32) alternatives by scale *
     scores, equal ones by the lower index.  A row with every score masked has log
     probabilities of -inf and entropy 0; a row with a NaN or scale * score = +inf has NaN.
+    |scale| is at least 2^-120 (float16 2^-126, float64 2^-1014), at most 2^126 (float64 2^1022).
     Differentiable in scores through log_probs and entropy (not through the alternatives)."""
     scale, top = float(scale), int(top)
     if isinstance(scores, torch.Tensor) and scores.requires_grad and torch.is_grad_enabled():

@@ -351,8 +351,9 @@ typedef enum { EUC_ROW_F32 = 0, EUC_ROW_F64 = 1, EUC_ROW_F16 = 2, EUC_ROW_BF16 =
  *   row_stats[i, 3]  = what euc_label_log_probs_grad needs of the row
  * log_probs (with labels), entropy and row_stats are nullable.  z = -inf masks a score;
  * a row with none left has log probabilities of -inf and entropy 0, a row with a NaN or
- * z = +inf has NaN.  Outputs are fp32 (fp64 for fp64 scores).  |scale| is
- * finite and not 0, and in [2^-126, 2^126] but for fp64. */
+ * z = +inf has NaN.  Outputs are fp32 (fp64 for fp64 scores).  |scale| is in
+ * [2^-120, 2^126] for fp32 and bf16, [2^-126, 2^126] for fp16, [2^-1014, 2^1022] for
+ * fp64. */
 EUC_API int euc_label_log_probs(int row_type, const void* scores, int64_t ld, int64_t n, int64_t m, const void* labels,
                         int labels_are_i64, double scale, int top, void* log_probs, void* entropy,
                         void* row_stats, void* top_log_probs, int64_t* top_labels, void* stream);
