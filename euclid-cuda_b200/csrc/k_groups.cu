@@ -779,6 +779,7 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
 #pragma unroll
               for (int e = 0; e < N; ++e) dot[j] += to_acc(g[q].e[e]) * to_acc(z[q][j].e[e]);
             }
+          if (gZ)
 #pragma unroll
           for (int j = 0; j < J; ++j)
             if (r[j] >= 0) {
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(256) rows_from_groups_grad_kernel(
       }
     }
   }
-  zero_rows(gZr, *kept, slots, nv, blockIdx.x, gridDim.x);
+  if (gZ) zero_rows(gZr, *kept, slots, nv, blockIdx.x, gridDim.x);
 }
 
 // ------------------------------------------------------------------ launches

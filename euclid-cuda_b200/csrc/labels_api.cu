@@ -185,8 +185,8 @@ int euc_rows_from_groups_grad(int row_type, const void* grad_out, const void* Y,
   if (int rc = bad_type(row_type)) return rc;
   if (int rc = rows_shape(n, p, dim)) return rc;
   if (int rc = no_device()) return rc;
-  if (n == 0 || p == 0) return EUC_OK;
-  if (!position || !kept || (dim > 0 && (!grad_out || !grad_Y || (grad_weights && !Y))))
+  if (n == 0 || p == 0 || (!grad_Y && !grad_weights)) return EUC_OK;
+  if (!position || !kept || (dim > 0 && (!grad_out || (grad_weights && !Y))))
     return set_error(EUC_ERR_ARG, "null pointer");
   if (misaligned(row_type, {grad_out, Y, grad_Y}, {weights, grad_weights}, {position, kept}, nullptr, false))
     return set_error(EUC_ERR_ARG, "misaligned pointer");

@@ -121,15 +121,24 @@ def rows_from_groups_grad(grad_out, Y, groups, weights=None):
     """Gradients of rows_from_groups: (grad_Y, grad_weights), the second None without
     weights.  grad_Y[position[i, j]] = weights[i, j] * grad_out[i], zero rows behind the
     last kept slot; grad_weights[i, j] = <grad_out[i], Y[position[i, j]]>, 0 where dropped."""
-    n, p, k = check_groups(groups)
-    rt, d = _check_rows(Y, "Y", n * p, groups)
+    n, p, _ = check_groups(groups)
+    _, d = _check_rows(Y, "Y", n * p, groups)
     _check_weights(weights, Y, groups)
     _ops.check_like(grad_out, "grad_out", (n, d), Y.dtype, Y.device)
-    grad_Y = torch.empty_like(Y)
-    grad_w = torch.empty_like(weights) if weights is not None else None
-    call_on(Y, lib().euc_rows_from_groups_grad, rt, grad_out.data_ptr(), Y.data_ptr(), groups.position.data_ptr(),
-            weights.data_ptr() if weights is not None else None, _kept(groups, k), n, p, d, grad_Y.data_ptr(),
-            grad_w.data_ptr() if weights is not None else None)
+    return _from_groups_grad(grad_out, Y, groups, weights, True, weights is not None)
+
+
+def _from_groups_grad(grad_out, Y, groups, weights, want_Y, want_weights):
+    """The wanted ones of (grad_Y, grad_weights), None for the other; grad_Y needs the
+    weights (None for ones), grad_weights needs Y."""
+    n, p, k = check_groups(groups)
+    rt, d = _check_rows(grad_out, "grad_out", n, groups)
+    grad_Y = grad_out.new_empty((n * p, d)) if want_Y else None
+    grad_w = grad_out.new_empty(groups.position.shape, dtype=_ops.acc_dtype(grad_out)) if want_weights else None
+    call_on(grad_out, lib().euc_rows_from_groups_grad, rt, grad_out.data_ptr(),
+            Y.data_ptr() if want_weights else None, groups.position.data_ptr(),
+            weights.data_ptr() if weights is not None else None, _kept(groups, k), n, p, d,
+            grad_Y.data_ptr() if want_Y else None, grad_w.data_ptr() if want_weights else None)
     return grad_Y, grad_w
 
 
@@ -150,14 +159,17 @@ class _FromGroups(torch.autograd.Function):
     @staticmethod
     def forward(ctx, Y, groups, weights):
         out = _from_groups(Y, groups, weights)
-        ctx.save_for_backward(Y, weights, *groups)
+        # each gradient needs the other input: Y, the largest tensor, is kept for the weights' alone
+        need_Y, _, need_weights = ctx.needs_input_grad
+        ctx.save_for_backward(Y if need_weights else None, weights if need_Y else None, *groups)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         Y, weights, *groups = ctx.saved_tensors
-        grad_Y, grad_w = rows_from_groups_grad(g.contiguous(), Y, RowGroups(*groups), weights)
+        need_Y, _, need_weights = ctx.needs_input_grad
+        grad_Y, grad_w = _from_groups_grad(g.contiguous(), Y, RowGroups(*groups), weights, need_Y, need_weights)
         return grad_Y, None, grad_w
 
 

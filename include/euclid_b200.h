@@ -386,8 +386,9 @@ EUC_API int euc_rows_to_groups(int row_type, const void* X, const int32_t* posit
 EUC_API int euc_rows_from_groups(int row_type, const void* Y, const int32_t* position, const void* weights, int64_t n,
                          int64_t p, int64_t dim, void* out, void* stream);
 /* Gradients of euc_rows_from_groups: grad_Y[position[i, j]] = weights[i, j] grad_out[i]
- * (zero rows behind the last kept slot) and, if grad_weights is not null,
- * grad_weights[i, j] = <grad_out[i], Y[position[i, j]]> (0 where dropped). */
+ * (zero rows behind the last kept slot) and
+ * grad_weights[i, j] = <grad_out[i], Y[position[i, j]]> (0 where dropped); either is
+ * nullable, and Y is read for grad_weights alone. */
 EUC_API int euc_rows_from_groups_grad(int row_type, const void* grad_out, const void* Y, const int32_t* position,
                               const void* weights, const int32_t* kept, int64_t n, int64_t p, int64_t dim,
                               void* grad_Y, void* grad_weights, void* stream);
