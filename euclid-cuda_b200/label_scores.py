@@ -75,6 +75,7 @@ class _LogProbs(torch.autograd.Function):
         r = _forward(scores, labels, scale, top)
         ctx.save_for_backward(scores, labels, r.row_stats)
         ctx.scale = scale
+        ctx.set_materialize_grads(False)  # an output that the loss leaves out costs nothing
         ctx.mark_non_differentiable(r.top_log_probs, r.top_labels, r.row_stats)
         return tuple(r)
 
@@ -82,8 +83,8 @@ class _LogProbs(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_log_probs, g_entropy, *_):
         scores, labels, stats = ctx.saved_tensors
-        if labels is None:
-            g_log_probs = None
+        if g_log_probs is None and g_entropy is None:
+            return None, None, None, None
         g = label_log_probs_grad(scores, labels, stats,
                                  g_log_probs.contiguous() if g_log_probs is not None else None,
                                  g_entropy.contiguous() if g_entropy is not None else None, ctx.scale)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import label_scores
 from row_groups import group_rows, rows_from_groups, rows_from_groups_grad
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +78,26 @@ def test_one_gradient_at_a_time(n, p, d, dtype):
     a.grad = b.grad = None
     rows_from_groups(a, groups, b).backward(G)
     assert torch.equal(a.grad, want[0]) and torch.equal(b.grad, want[1])
+
+
+def test_outputs_outside_the_loss_cost_nothing(monkeypatch):
+    """A loss through one output alone: no gradient of zeros for the other is made or read."""
+    seen = []
+    real = label_scores.label_log_probs_grad
+
+    def spy(scores, labels, stats, grad_log_probs=None, grad_entropy=None, scale=1.0):
+        seen.append((grad_log_probs is not None, grad_entropy is not None))
+        return real(scores, labels, stats, grad_log_probs, grad_entropy, scale)
+    monkeypatch.setattr(label_scores, "label_log_probs_grad", spy)
+    x = torch.randn(50, 333, generator=gen(1), device="cuda").requires_grad_()
+    lab = torch.arange(50, device="cuda")
+    one = torch.ones(50, device="cuda")
+    for labels, pick, want in ((lab, lambda r: r.log_probs, (True, False)), (lab, lambda r: r.entropy, (False, True)),
+                               (None, lambda r: r.entropy, (False, True)),
+                               (lab, lambda r: r.log_probs + r.entropy, (True, True))):
+        x.grad = None
+        r = label_scores.label_log_probs(x, labels, 1.5, 2)
+        pick(r).sum().backward()
+        assert seen.pop() == want and not seen
+        assert torch.equal(x.grad, real(x.detach(), labels, r.row_stats, one if want[0] else None,
+                                        one if want[1] else None, 1.5))
