@@ -12,6 +12,7 @@ size limits (N*M <= 2^32, smem <= 48 KiB) do not exist here.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from _lib import OPS, check, exported_symbols, lib, ptr, stream_of, workspace
 
@@ -215,6 +216,16 @@ def row_type(t, name):
 def acc_dtype(t):
     """The type of sums, weights and statistics of rows of t's type."""
     return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def refuse_tangents(*tensors):
+    """The label operators have no forward-mode derivative: an input with a tangent is
+    refused (it does not require a gradient, and the output would come without one)."""
+    if forward_ad._current_level < 0:  # no dual level is open
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("forward-mode derivatives are not supported")
 
 
 def check_same_device(t, name, other, other_name):

@@ -14,6 +14,7 @@ from row_groups import check_groups, group_rows
 
 
 def _lookup(C, labels, scale):
+    _ops.refuse_tangents(C)
     _ops.check_input(C, "C")
     rt = _ops.row_type(C, "C")
     if C.dim() != 2:
@@ -31,6 +32,7 @@ def lookup_grad(G, labels, n_clusters, scale=1.0, groups=None):
     """grad_C [n_clusters, dim] in G's type: scale * the sum of G's rows with each label
     (G has the labels' shape and then dim; labels outside [0, n_clusters) add nothing, a
     label without rows gets zeros).  `groups`: the labels' group_rows, if the caller has it."""
+    _ops.refuse_tangents(G)
     _ops.check_input(G, "G")
     rt = _ops.row_type(G, "G")
     _ops.check_labels(labels)

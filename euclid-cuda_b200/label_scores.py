@@ -31,6 +31,7 @@ class LabelLogProbs(NamedTuple):
 def _check(scores, labels, scale):
     if not isinstance(scores, torch.Tensor):
         raise TypeError("scores must be a torch.Tensor")
+    _ops.refuse_tangents(scores)
     if not scores.is_cuda:
         raise RuntimeError("scores must be a CUDA tensor")
     if scores.dim() != 2:
@@ -110,6 +111,7 @@ def label_log_probs_grad(scores, labels, row_stats, grad_log_probs=None, grad_en
     forward call's.  Either gradient may be None; labels are needed with grad_log_probs."""
     scale = float(scale)
     n, m, ld, rt, i64 = _check(scores, labels, scale)
+    _ops.refuse_tangents(grad_log_probs, grad_entropy)
     acc = _ops.acc_dtype(scores)
     _ops.check_like(row_stats, "row_stats", (n, 3), acc, scores.device)
     if grad_log_probs is not None:

@@ -94,6 +94,7 @@ def _kept(groups, k):
 
 
 def _to_groups(X, groups):
+    _ops.refuse_tangents(X)
     n, p, k = check_groups(groups)
     rt, d = _check_rows(X, "X", n, groups)
     Y = X.new_empty((n * p, d))
@@ -108,6 +109,7 @@ def _check_weights(weights, Y, groups):
 
 
 def _from_groups(Y, groups, weights):
+    _ops.refuse_tangents(Y, weights)
     n, p, _ = check_groups(groups)
     rt, d = _check_rows(Y, "Y", n * p, groups)
     _check_weights(weights, Y, groups)
@@ -131,6 +133,7 @@ def rows_from_groups_grad(grad_out, Y, groups, weights=None):
 def _from_groups_grad(grad_out, Y, groups, weights, want_Y, want_weights):
     """The wanted ones of (grad_Y, grad_weights), None for the other; grad_Y needs the
     weights (None for ones), grad_weights needs Y."""
+    _ops.refuse_tangents(grad_out, Y, weights)
     n, p, k = check_groups(groups)
     rt, d = _check_rows(grad_out, "grad_out", n, groups)
     grad_Y = grad_out.new_empty((n * p, d)) if want_Y else None
