@@ -101,7 +101,12 @@ class LloydKMeans:
         """Soft assignment of the local rows: LabelLogProbs of -D / temperature, D the
         operator's squared distances, formed in blocks of `block_rows` rows (default:
         about 1 GiB of D) so that D is never whole.  `labels`: labels whose log
-        probabilities are wanted; `top`: the nearest centers per row, with theirs."""
+        probabilities are wanted; `top`: the nearest centers per row, with theirs.  Not
+        differentiable, as the distance operators are not: points or centers that require a
+        gradient are refused while gradients are recorded."""
+        _ops.refuse_tangents(X, C)
+        if torch.is_grad_enabled() and (X.requires_grad or C.requires_grad):
+            raise RuntimeError("posterior is not differentiable: detach X and C, or call it under torch.no_grad()")
         if not temperature > 0:
             raise RuntimeError("temperature must be positive")
         n, m = X.size(0), C.size(0)
