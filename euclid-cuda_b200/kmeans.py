@@ -112,6 +112,8 @@ class LloydKMeans:
         n, m = X.size(0), C.size(0)
         if labels is not None and tuple(labels.shape) != (n,):
             raise RuntimeError(f"labels must have shape {(n,)}")
+        if block_rows is not None and int(block_rows) < 0:
+            raise RuntimeError("block_rows must not be negative")
         rows = int(block_rows) if block_rows else max(1, (1 << 30) // max(1, m * X.element_size()))
         parts = []
         for lo in range(0, n, rows) if n > 0 else (0,):

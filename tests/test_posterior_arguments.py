@@ -19,6 +19,11 @@ def test_gradients_are_refused():
         km.posterior(x, fwAD.make_dual(c, torch.ones_like(c)))
 
 
+def test_blocks_of_fewer_than_no_rows_are_refused():
+    with pytest.raises(RuntimeError, match="block_rows"):
+        LloydKMeans(2).posterior(torch.zeros(4, 3), torch.zeros(2, 3), block_rows=-5)
+
+
 @pytest.mark.gpu
 def test_without_recorded_gradients():
     g = torch.Generator(device="cuda").manual_seed(1)
