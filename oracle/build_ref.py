@@ -22,7 +22,8 @@ ref_center_kernels     center_kernels.cu (its PYBIND11_MODULE is in the .cu, cen
 Usage:  python oracle/build_ref.py [--src DIR] [--only NAME ...]
 
 The sources are read from --src, else $EUCLID_REFERENCE_SRC, else the reference checkout
-beside this repository (../reference); without them the recipe skips itself.
+beside this repository (../reference); without any of them the recipe skips itself, and
+with some of them missing it fails.
 """
 import argparse
 import os
@@ -77,13 +78,17 @@ def main():
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
-    if not all(os.path.isfile(os.path.join(a.src, f)) for fs in EXTENSIONS.values() for f in fs):
+    names = a.only or list(EXTENSIONS)
+    missing = {f for n in names for f in EXTENSIONS[n] if not os.path.isfile(os.path.join(a.src, f))}
+    if all(f in missing for n in names for f in EXTENSIONS[n]):
         print(f"[build_ref] reference sources not found at {a.src}; skipping")
         return 0
+    if missing:
+        print(f"[build_ref] incomplete reference sources at {a.src}: no {', '.join(sorted(missing))}", file=sys.stderr)
+        return 1
     os.makedirs(OUT, exist_ok=True)
     # torch's extension builder refuses to run without an arch list when no GPU is visible
     os.environ.setdefault("TORCH_CUDA_ARCH_LIST", "10.0a")
-    names = a.only or list(EXTENSIONS)
     for n in names:
         if built(n) and not a.force:
             print(f"[build_ref] {n}: up to date")
