@@ -101,7 +101,8 @@ class LloydKMeans:
         """Soft assignment of the local rows: LabelLogProbs of -D / temperature, D the
         operator's squared distances, formed in blocks of `block_rows` rows (default:
         about 1 GiB of D) so that D is never whole.  `labels`: labels whose log
-        probabilities are wanted; `top`: the nearest centers per row, with theirs.  Not
+        probabilities are wanted; `top`: the nearest centers per row, with theirs.  With more
+        than 1024 centers the last bits may depend on how many rows a block has.  Not
         differentiable, as the distance operators are not: points or centers that require a
         gradient are refused while gradients are recorded."""
         _ops.refuse_tangents(X, C)
