@@ -366,9 +366,10 @@ __device__ __forceinline__ void both(const Sums<double>& p, double& s, double& t
 // bound), a better bound is looked for: a block takes the last place among those it holds, a
 // team halves the range of values.  Scores that are equal beyond the list's size bound
 // themselves: those above them are listed, and the places left go to the first of the equal
-// ones.  A NaN takes the plain way: the best one behind the last one, `top` times.
+// ones.  A row with a NaN has its first ones first, and then the best one behind the last one, a
+// pass over the row each.
 // (50 scores side by side, all others masked by -1e4, the 20 best: 4096 x 131072 bf16 0.23 ms,
-// 131072 x 1024 fp32 0.47; by the plain way 41.7 and 5.5.)
+// 131072 x 1024 fp32 0.47; by a pass over the row for each 41.7 and 5.5.)
 
 // The q-th largest over the team's lanes of each list, the smallest over the lists: q - 1
 // rounds strike each list's largest (and its equals, which only lowers the bound).  No NaN.
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) =
       }
     }
     const bool over = !slow && count > CAP;
-    const bool odd = __any_sync(0xffffffffu, over || (!slow && count < a.top));
+    const bool odd = __any_sync(0xffffffffu, over || slow || count < a.top);
     A tie = neg_inf<A>();  // the places that the listed scores leave go to the first that equal it
     if (odd && __any_sync(0xffffffffu, over)) {
       // More than the list holds: a value that at least `top` scores reach and the list holds is
@@ -609,55 +610,47 @@ __global__ void __launch_bounds__(128, EPL * sizeof(Acc<T>) > 128 ? (sizeof(T) =
     }
     if (!early && more) fetch(first + step + team);
     if (odd) {
-      // the first that equal `tie`: masked ones where t is the lowest number
-      bool fill = !slow && count < a.top;
+      // the first that equal `tie`: masked ones where t is the lowest number; of a row with a NaN
+      // the first NaN
+      __syncwarp();  // the list's first entries are in, before some are written again
+      if (slow) count = 0;
+      bool fill = count < a.top;
       for (int j0 = 0; __any_sync(0xffffffffu, fill); j0 += TEAM) {
         const int j = j0 + tl;
-        const bool here = fill && j < a.m && row.at(j) == tie;
+        const A z = fill && j < a.m ? row.at(j) : A(0);
+        const bool here = fill && j < a.m && (slow ? z != z : z == tie);
         const unsigned b = __ballot_sync(0xffffffffu, here);
         const int at = count + __popc(b & before_me);
-        if (here && at < a.top) list[at] = Key<A>::of(tie, j);
+        if (here && at < a.top) list[at] = Key<A>::of(z, j);
         if (fill) count = min(count + __popc(b & team_lanes), a.top);
         fill = fill && count < a.top && j0 + TEAM < a.m;
       }
+      // and then, of such a row, the best one behind the last one
+      while (__any_sync(0xffffffffu, slow && count < a.top)) {
+        __syncwarp();
+        const Key<A> last = list[max(count - 1, 0)];
+        Key<A> best = Key<A>::none();
+        for (int j = tl; j < a.m; j += TEAM) {
+          const Key<A> o = Key<A>::of(row.at(j), j);
+          if (last.ahead(o) && o.ahead(best)) best = o;
+        }
+#pragma unroll
+        for (int s = TEAM / 2; s > 0; s >>= 1) {
+          const Key<A> o = best.other(s);
+          if (o.ahead(best)) best = o;
+        }
+        if (slow && count < a.top) {
+          if (tl == 0) list[count] = best;
+          ++count;
+        }
+      }
     }
     __syncwarp();
-    if (!slow && live) {
+    if (live) {
       for (int q = tl; q < count; q += TEAM) {
         const Key<A> me = list[q];
         const int place = place_of(list, count, me);
         if (place < a.top) write_top(a, i, place, me, hi, L);
-      }
-    }
-    if (__any_sync(0xffffffffu, slow)) {
-      // a NaN: the best one behind the last one; after it the next equal one, if there is any,
-      // which is the first such score behind it
-      Key<A> last = Key<A>::none();
-      int from = a.m;  // where the next equal one is looked for
-      for (int k = 0; k < a.top; ++k) {
-        Key<A> best = Key<A>::none();
-        for (int j0 = from; __any_sync(0xffffffffu, j0 < a.m && best.order() == 0); j0 += TEAM) {
-          const int j = j0 + tl;
-          const bool equal = best.order() == 0 && j < a.m && order_of(row.at(j)) == last.order();
-          const unsigned b = __ballot_sync(0xffffffffu, equal) & team_lanes;
-          if (b != 0u) best = Key<A>::of(last.y(), j0 + (__ffs(b) - 1) % TEAM);
-        }
-        if (__any_sync(0xffffffffu, best.order() == 0)) {
-          Key<A> other = Key<A>::none();
-          for (int j = tl; j < a.m; j += TEAM) {
-            const Key<A> o = Key<A>::of(row.at(j), j);
-            if ((k == 0 || last.ahead(o)) && o.ahead(other)) other = o;
-          }
-#pragma unroll
-          for (int s = TEAM / 2; s > 0; s >>= 1) {
-            const Key<A> o = other.other(s);
-            if (o.ahead(other)) other = o;
-          }
-          if (best.order() == 0) best = other;
-        }
-        last = best;
-        from = best.j() + 1;
-        if (tl == 0 && slow && live) write_top(a, i, k, best, hi, L);
       }
     }
     __syncwarp();
@@ -924,8 +917,9 @@ __global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1)
       __syncthreads();
     }
     // the first that equal `tie` (masked ones where the bound is the lowest number), a vector a
-    // thread and turn
-    for (int v = slow ? v1 : v0; found < want && v < v1; v += NT) {
+    // thread and turn; of a slice with a NaN the first NaN
+    if (slow) found = 0;
+    for (int v = v0; found < want && v < v1; v += NT) {
       uint32_t here = 0u;
       if (v + static_cast<int>(threadIdx.x) < v1) {
         A y[VE];
@@ -933,7 +927,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const int j = (v + static_cast<int>(threadIdx.x)) * VE - row.off + e;
-          here |= y[e] == tie && j >= j0 && j < j1 ? 1u << e : 0u;
+          here |= (slow ? y[e] != y[e] : y[e] == tie) && j >= j0 && j < j1 ? 1u << e : 0u;
         }
       }
       int before = __popc(here);
@@ -953,49 +947,38 @@ __global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1)
         all += equals[w];
       }
       for (int place = found + before; here != 0u && place < want; ++place) {
-        list[place] = Key<A>::of(tie, (v + static_cast<int>(threadIdx.x)) * VE - row.off + __ffs(here) - 1);
+        list[place] = Key<A>::of(slow ? hi : tie, (v + static_cast<int>(threadIdx.x)) * VE - row.off + __ffs(here) - 1);
         here &= here - 1u;
       }
       found += all;
     }
-    if (slow) {
-      // a NaN: the best one behind the last one; after it the next equal one, if there is any,
-      // which is the first such score behind it
-      Key<A> last = Key<A>::none();
-      int from = j1;  // where the next equal one is looked for
-      for (int k = 0; k < want; ++k) {
-        Key<A> best = Key<A>::none();
-        for (int s = from; s < j1 && best.order() == 0; s += NT) {
-          const int j = s + static_cast<int>(threadIdx.x);
-          const bool equal = j < j1 && order_of(row.at(j)) == last.order();
-          const unsigned b = __ballot_sync(0xffffffffu, equal);
-          __syncthreads();
-          if (lane == 0) cands[warp] = b != 0u ? Key<A>::of(last.y(), s + warp * 32 + __ffs(b) - 1) : Key<A>::none();
-          __syncthreads();
+    // and then, of such a slice, the best one behind the last one
+    for (; slow && found < want; ++found) {
+      __syncthreads();
+      const Key<A> last = list[max(found - 1, 0)];
+      Key<A> best = Key<A>::none();
+      for (int v = v0 + static_cast<int>(threadIdx.x); v < v1; v += NT) {
+        A y[VE];
+        row.load(v, y);
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (cands[w].ahead(best)) best = cands[w];
+        for (int e = 0; e < VE; ++e) {
+          const int j = v * VE - row.off + e;
+          const Key<A> o = Key<A>::of(y[e], j);
+          if (j >= j0 && j < j1 && last.ahead(o) && o.ahead(best)) best = o;
         }
-        if (best.order() == 0) {
-          for (int j = j0 + static_cast<int>(threadIdx.x); j < j1; j += NT) {
-            const Key<A> o = Key<A>::of(row.at(j), j);
-            if ((k == 0 || last.ahead(o)) && o.ahead(best)) best = o;
-          }
+      }
 #pragma unroll
-          for (int s = 16; s > 0; s >>= 1) {
-            const Key<A> o = best.other(s);
-            if (o.ahead(best)) best = o;
-          }
-          __syncthreads();
-          if (lane == 0) cands[warp] = best;
-          __syncthreads();
+      for (int s = 16; s > 0; s >>= 1) {
+        const Key<A> o = best.other(s);
+        if (o.ahead(best)) best = o;
+      }
+      if (lane == 0) cands[warp] = best;
+      __syncthreads();
+      if (threadIdx.x == 0) {
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (cands[w].ahead(best)) best = cands[w];
-        }
-        last = best;
-        from = best.j() + 1;
-        if (threadIdx.x == 0) list[k] = best;
+        for (int w = 1; w < W; ++w)
+          if (cands[w].ahead(best)) best = cands[w];
+        list[found] = best;
       }
     }
   }

@@ -93,3 +93,38 @@ def test_finite_masks_cost_what_other_rows_cost(n, m, dtype, kept, top):
     x[:, m // 3 + kept:] = -1e4
     finite = median_us(lambda: label_log_probs(x, None, 1.0, top))
     assert finite <= 6 * plain, (finite, plain)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,top", [(40, 8), (250, 20), (500, 16), (1000, 20), (1021, 5), (2000, 8), (3000, 32), (9001, 4),
+                                   (70001, 20)])
+def test_rows_with_nan(m, top, dtype):
+    """One NaN, a few, fewer than the alternatives or more, in one part of the row or throughout,
+    among others, masked ones and equal ones: the NaN first, by index, then the others."""
+    x = torch.randn(9, m, generator=gen(m), device="cuda").to(dtype)
+    x[0, m // 2] = math.nan
+    x[1, 1::2] = math.nan
+    x[2, m - 3:] = math.nan
+    x[3] = math.nan
+    x[4] = -math.inf
+    x[4, m // 3], x[4, 2] = math.nan, 1.0
+    x[5] = 0.25
+    x[5, m - 1] = math.nan
+    x[6, 0], x[6, 1] = math.nan, math.inf
+    x[7] = -1e4
+    x[7, 3], x[7, m - 2] = math.nan, 0.5
+    lab = torch.arange(9, device="cuda")
+    check(x, lab, 1.0, top, grads=False)  # (row 8 has none)
+    check(-x, lab, -1.0, top, grads=False)
+    many = x.repeat(150, 1)
+    r, few = label_log_probs(many, None, 1.0, top), label_log_probs(x, None, 1.0, top)
+    assert torch.equal(r.top_labels, few.top_labels.repeat(150, 1))
+
+
+@pytest.mark.parametrize("n,m,dtype", [(4096, 131072, torch.bfloat16), (65536, 3000, torch.bfloat16)])
+def test_rows_of_nan_cost_what_other_rows_cost(n, m, dtype):
+    """A training step that has gone wrong: nothing but NaN (six times as above)."""
+    x = torch.randn(n, m, generator=gen(m), device="cuda", dtype=torch.float32).to(dtype)
+    plain = median_us(lambda: label_log_probs(x, None, 1.0, 20))
+    x.fill_(math.nan)
+    assert median_us(lambda: label_log_probs(x, None, 1.0, 20)) <= 6 * plain
