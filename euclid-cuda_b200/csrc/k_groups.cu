@@ -17,8 +17,8 @@
 // 2.8 us.  More take three kernels a pass (histograms of tiles, scan of each bin over the
 // tiles, scatter through shared memory so that a bin's run is stored together): 131072 slots
 // of 128 labels in 6.3 us (one cluster of 8 blocks took 54: eight SMs scatter no faster),
-// 8192 of 256 in 6.8 (one block: 23).  The sort moves 4 to 8 bytes a slot where the rows move
-// kilobytes.
+// 8192 of 256 in 6.8 (one block: 23).  One pass reads a slot's label twice and writes its three
+// results, 20 to 28 bytes a slot, each further pass about as many again; the rows move kilobytes.
 //
 // The row kernels are bound by HBM, and read and write every row once: a row's copies are
 // written from registers after one read, its weighted sum is formed from p reads (16384 rows
@@ -36,8 +36,10 @@ namespace euc {
 // k + 1 bins (the last for labels outside [0, k)) that one pass may have: of a block, and of
 // three kernels, what shared memory holds per warp and bin; of more than kManySlots slots,
 // what their histograms cost (262144 of 2900 labels: 22 us in one pass, 27 in two; 1048576 of
-// 4000: 94 in one, 50 in two).  30011 of 4099 take 25 us in one pass and 18.6 in two, but
-// the four launches more cost the host 5 us more than that.
+// 4000: 94 in one, 50 in two).  Below kManySlots the limit weighs the device against the host's
+// four launches more: 5000 to 60000 slots of 2100, 3100 and 4600 labels take 16 to 20, 18 to 25
+// and 21 to 31 us in one pass and 17 to 19 in two as part of a captured graph, but 24 to 26, 24
+// to 31 and 27 to 35 in one and 33 in two as calls of their own.
 constexpr int kBlockBins = 2049;
 constexpr int kMaxBins = 4609;
 constexpr int kManyBins = 1537;
@@ -85,7 +87,7 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int m, uint32_t* warp_su
 // rank[u] <- slots of the warp before (u, lane) with its digit; counts <- slots per digit.
 // The lanes with a lane's digit come from a ballot per bit: match_any, whose lanes take turns,
 // costs more from a few labels up (1048576 slots of 4, 64 and 1024: 12.6, 18.4 and 26.7 us with
-// it, 13.4, 14.9 and 23.2 so).
+// it, 13.9, 15.9 and 24.5 so).
 template <int ITEMS>
 __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], unsigned short (&rank)[ITEMS],
                                            unsigned short* counts, int lane, int bits) {
@@ -380,7 +382,7 @@ struct SortPlan {
 
 // Tiles: small ones fill the SMs, and are cheap to begin while the bins are few; large ones
 // leave fewer histograms to add up (131072 slots of 128 labels: 6.3, 7.5 and 9.5 us with
-// 8 x 4, 16 x 4 and 16 x 8; 65536 of 1024: 13.3, 14.1, 19.2; 1048576 of 1024: 36, 32, 25).
+// 8 x 4, 16 x 4 and 16 x 8; 65536 of 1024: 13.3, 14.1, 19.2; 1048576 of 1024: 36, 32, 24.5).
 // Where only 16 x 4 are at most one per SM, their kernels overlap (200000 of 128: 9.5, 7.5, 9.5).
 constexpr int64_t kSmsOfB200 = 148;
 

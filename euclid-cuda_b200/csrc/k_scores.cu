@@ -15,10 +15,10 @@
 // NaN counts as the largest value.
 //
 // The scores are read once, so HBM is the bound: 131072 x 1024 fp32 without alternatives take
-// 84 us (6.4 TB/s), 4096 x 131072 bf16 180 (6.0).  The alternatives cost instructions, some
-// hundreds a row whatever its length: with the 8 best the first takes 131 us, bound by issue,
-// with the 20 best the second 209.  One row of 131072 is bound by latency: 4.5 us, 11 with 20
-// alternatives.
+// 85 us (6.3 TB/s), 4096 x 131072 bf16 179 (6.0).  The alternatives cost instructions, some
+// hundreds a row whatever its length: with the 8 best the first takes 132 us (840 instructions a
+// row and warp, the issue slots 76 % busy, HBM 50 %), with the 20 best the second 205.  One row
+// of 131072 is bound by latency: 4.9 us, 10.5 with 20 alternatives.
 #include "common.cuh"
 #include "engine.h"
 #include "rows.cuh"
