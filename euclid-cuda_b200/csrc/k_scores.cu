@@ -845,7 +845,9 @@ __global__ void __launch_bounds__(NT, sizeof(T) <= 4 ? 1024 / NT : 1)
     A tie = neg_inf<A>();  // the places that the listed scores leave go to the first that equal it
     bool above = false;    // whether the bound is the next number above `tie`
     int found = want;
-    while (!slow) {
+    // Two turns that do not list all leave out at least 256 - kMaxTop of the slice's scores: the
+    // limit is never reached, unless the scores change while they are read.
+    for (int turns = (j1 - j0) / 64 + 8; !slow && turns > 0; --turns) {
       auto add = [&](A y, int j) {
         const int at = atomicAdd(&count_sh, 1);
         if (at < kBlockCands) cands[at] = Key<A>::of(y, j);
