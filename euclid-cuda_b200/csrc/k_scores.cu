@@ -1261,9 +1261,9 @@ template <typename T> static cudaError_t scores_t(const ScoreJob& j, cudaStream_
   if constexpr (sizeof(T) < 8)
     if (a.m <= 2048 && a.n >= num_sms() * 4 && rows_are_vectors(a)) return scores_team<T, 32, 64>(a, st);
   // Small blocks for short rows of which there are enough: what a block does once a row costs
-  // every one of its warps (65536 x 3000 bf16 top 8: 211 us with 32 threads, 259 with 64, 349
-  // with 128), long rows need their vectors in flight (16384 x 8192 fp32: 131, 105 and 123;
-  // 4096 x 131072 bf16 top 20: 209 with 128 and 223 with 256).
+  // every one of its warps (65536 x 3000 bf16 top 8: 227 us with 32 threads, 253 with 64, 343
+  // with 128), long rows need their vectors in flight (16384 x 8192 fp32 top 8: 137, 110 and 133;
+  // 4096 x 131072 bf16 top 20: 204 with 128 and 215 with 256).
   const int64_t bytes = static_cast<int64_t>(a.m) * static_cast<int64_t>(sizeof(T));
   if (bytes <= 8192 && a.n >= num_sms() * 8) return scores_block<T, 32>(a, st);
   if (bytes <= 32768 && a.n >= num_sms() * 8) return scores_block<T, 64>(a, st);
